@@ -1,0 +1,661 @@
+"""The paged KV cache on the GPU (include/hk_paged.h) against the float64 oracle.
+
+Tolerances of the attention, per output o = sum_j p_j v_j (p the probabilities, A = sum_j p_j |v_j|):
+
+- the result's rounding to bf16: 2^-8 |o| (half a step relative to the value, eps / 2)
+- each probability's rounding to bf16 before its product: 2^-8 A
+- a score's float32 error e_s moves p_j by e_s p_j relative, at most 2 e_s with the sum's share: 2 e_s A, where
+  e_s <= D 2^-24 max|q||k| scale (a sum of D exact products, each partial sum rounded) + 2^-23 |s| for the scaling
+- exp2 and the sum of the probabilities: a few 2^-23, below 2^-18 A for up to 8192 slots in runs
+
+Inputs are drawn once; NaN in a place that a row does not see has to leave no trace at all."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from _util import announce
+from oracle import bf16
+from oracle import paged as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _bits(x):
+    return bf16.to_bits(np.asarray(x, np.float32))
+
+
+def _floats(bits):
+    return bf16.from_bits(bits).astype(np.float64)
+
+
+class Cache:
+    """The oracle's cache and the same on the GPU."""
+
+    def __init__(self, rng, *, layers=1, pages, kv_heads, page, dim, seqs, width, e4m3=False, gap=0, poison=True):
+        from runtime import hip, paged
+
+        self.e4m3, self.dim, self.page = e4m3, dim, page
+        shape = (layers, pages, kv_heads, page, dim)
+        self.scale = {x: rng.uniform(0.01, 0.03, (layers, kv_heads)).astype(np.float32) for x in "kv"}
+        self.o = {"table": np.full((seqs, width), -1, np.int32), "length": np.zeros(seqs, np.int32),
+                  "refs": np.zeros(pages, np.int32)}
+        # every slot starts as NaN: whatever is read without having been written shows
+        start = np.full(shape, np.nan if poison else 0.0)
+        self.o["k"], self.o["v"] = start, start.copy()
+        self.stride = kv_heads * page * dim + gap
+        self.c = paged.PagedCache(layers=layers, kv_heads=kv_heads, head_dim=dim, page_size=page, pages=pages, seqs=seqs,
+                                  table_width=width, dtype=paged.E4M3 if e4m3 else paged.BF16,
+                                  page_stride=self.stride, layer_stride=pages * self.stride + gap)
+        self.bufs = {"workspace": hip.DeviceBuffer(paged.WORKSPACE)}
+        self.bufs["workspace"].zero()
+        self.upload()
+        if e4m3:
+            for x in "kv":
+                self.bufs[x + "_scale"] = hip.DeviceBuffer.from_array(self.scale[x])
+                setattr(self.c, x + "_scale", self.bufs[x + "_scale"].ptr)
+
+    def encode(self, x, which, layer):
+        """Rows [.., kv heads, .., dim] as the pool's numbers; ``x`` has the heads on axis 1."""
+        if not self.e4m3:
+            return _bits(x)
+        s = self.scale[which][layer].reshape(1, -1, 1, 1)
+        return oracle.e4m3(np.asarray(x, np.float32) / s)
+
+    def decode(self, codes, which, layer):
+        if not self.e4m3:
+            return _floats(codes)
+        return oracle.from_e4m3(codes) * self.scale[which][layer].astype(np.float64).reshape(1, -1, 1, 1)
+
+    def store(self, layer):
+        """The oracle's rounding of appended rows."""
+        def f(rows, which):
+            x = np.asarray(rows)[None, :, None, :]
+            return self.decode(self.encode(x.astype(np.float32), which, layer), which, layer)[0, :, 0]
+        return f
+
+    def _pool(self, which):
+        layers, pages = self.o["k"].shape[:2]
+        kind = np.uint8 if self.e4m3 else np.uint16
+        flat = np.full(layers * self.c.layer_stride, 0x7F if self.e4m3 else 0x7FC0, kind)
+        for l in range(layers):
+            rows = flat[l * self.c.layer_stride:][:pages * self.stride].reshape(pages, self.stride)
+            rows[:, :self.o["k"][l, 0].size] = self.encode(self.o[which][l], which, l).reshape(pages, -1)
+        return flat
+
+    def upload(self):
+        from runtime import hip
+
+        for x in ("k", "v", "table", "length", "refs"):
+            if x in self.bufs:
+                self.bufs[x].free()
+            self.bufs[x] = hip.DeviceBuffer.from_array(self._pool(x) if x in "kv" else self.o[x])
+            setattr(self.c, x, self.bufs[x].ptr)
+
+    def download(self, which, layer):
+        layers, pages, heads, page, dim = self.o["k"].shape
+        flat = self.bufs[which].read(np.uint8 if self.e4m3 else np.uint16, layers * self.c.layer_stride)
+        rows = flat[layer * self.c.layer_stride:][:pages * self.stride].reshape(pages, self.stride)
+        return rows[:, :heads * page * dim].reshape(pages, heads, page, dim)
+
+    def fill(self, rng, layer=0):
+        """Normal keys and values, as the pool holds them, in the slots below each length; all others stay."""
+        for s, n in enumerate(self.o["length"]):
+            slot, page, at = oracle.slots_of(self.o, s, oracle.length_of(self.o, s))
+            for x in "kv":
+                new = rng.normal(size=(1, self.o["k"].shape[2], len(slot), self.dim)).astype(np.float32)
+                got = self.decode(self.encode(new, x, layer), x, layer)[0]
+                self.o[x][layer, page, :, at] = got.transpose(1, 0, 2)
+
+    def give(self, lengths, rng):
+        """Pages in a random order to sequences of these lengths."""
+        free = list(rng.permutation(np.flatnonzero(self.o["refs"] == 0)))
+        for s, n in enumerate(lengths):
+            for j in range(-(-n // self.page)):
+                self.o["table"][s, j] = free.pop()
+                self.o["refs"][self.o["table"][s, j]] = 1
+            self.o["length"][s] = n
+
+
+def _dev(array):
+    from runtime import hip
+
+    return hip.DeviceBuffer.from_array(np.ascontiguousarray(array))
+
+
+def _sync():
+    from runtime import hip
+
+    hip.check(hip.lib().hk_stream_sync(None), "sync")
+
+
+def attention(cache, layer, q_bits, seqs, first, *, scale, window=0, max_new=None, stride=None, want_lse=True,
+              stream=None):
+    """(out [tokens, heads, dim] float64, lse, raw out bits): memory of rows that the call leaves alone reads as the
+    pattern 0x4242."""
+    from runtime import hip, paged
+
+    tokens, heads, dim = q_bits.shape
+    width = heads * dim
+    stride = stride or width
+    q = np.full((tokens + 1, stride), 0x7FC0, np.uint16)
+    q[:tokens, :width] = q_bits.reshape(tokens, width)
+    Q, S, F = _dev(q), _dev(np.asarray(seqs, np.int32)), _dev(np.asarray(first, np.int32))
+    O, L = _dev(np.full((tokens + 1, stride), 0x4242, np.uint16)), _dev(np.full((tokens, heads), 77, np.float32))
+    if max_new is None:
+        max_new = max(1, int(np.diff(first).max(initial=1)))
+    hip.check(paged.lib().hk_paged_attention(
+        ctypes.byref(cache.c), layer, Q.ptr, stride, S.ptr, F.ptr, len(seqs), tokens, max_new, heads, scale, window, O.ptr,
+        stride, L.ptr if want_lse else None, cache.bufs["workspace"].ptr, stream), "hk_paged_attention")
+    hip.check(hip.lib().hk_stream_sync(stream), "sync")
+    raw = O.read(np.uint16, (tokens + 1) * stride).reshape(tokens + 1, stride)
+    assert np.all(raw[tokens] == 0x4242) and np.all(raw[:, width:] == 0x4242), "written outside the rows"
+    raw = raw[:tokens, :width].reshape(tokens, heads, dim)
+    return _floats(raw), L.read(np.float32, tokens * heads).reshape(tokens, heads), raw
+
+
+def check_attention(got, lse, raw, want, q, cache, scale):
+    out, want_lse, spread = want
+    mine = spread[:, :, 0] != -1
+    assert np.all(raw[~mine] == 0x4242), "rows of no entry were written"
+    assert np.all(lse[~mine] == 77)
+    dim = q.shape[2]
+    k = cache.o["k"]
+    top_k = np.abs(np.where(np.isfinite(k), k, 0)).max() * np.sqrt(dim)
+    e_s = dim * 2.0**-24 * np.linalg.norm(q, axis=-1)[mine] * top_k * scale * 1.01 + 2.0**-23 * 64
+    tol = 2.0**-8 * (np.abs(out[mine]) + spread[mine]) + (2 * e_s[:, None] + 2.0**-18) * spread[mine] + 1e-30
+    nan = np.isnan(out[mine])
+    np.testing.assert_array_equal(np.isnan(got[mine]), nan)
+    err = np.where(nan, 0, np.abs(got[mine] - out[mine]))
+    assert np.all((err <= tol) | nan), f"{(err > tol).sum()} outside, worst {np.nanmax(err / tol):.2f} of the tolerance"
+    fine = np.isfinite(want_lse[mine])
+    np.testing.assert_array_equal(lse[mine][~fine], want_lse[mine][~fine])
+    off = np.abs(lse[mine][fine] - want_lse[mine][fine])
+    assert np.all(off <= e_s[fine] + 2.0**-18 + 2.0**-22 * np.abs(want_lse[mine][fine])), off.max()
+
+
+# (name, q heads, kv heads, dim, page, e4m3, [(length, new rows)], window)
+CASES = [
+    ("one token", 14, 2, 64, 16, False, [(1, 1)], 0),
+    ("one token, 71 slots", 14, 2, 64, 16, False, [(71, 1)], 0),
+    ("tokens at the edges of pages and tiles", 9, 3, 64, 16, False,
+     [(n, 1) for n in (15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 255, 257)], 0),
+    ("the same, 128 wide", 4, 1, 128, 32, False, [(n, 1) for n in (1, 31, 32, 33, 63, 64, 65, 127, 129, 300)], 0),
+    ("the same, e4m3", 8, 2, 64, 64, True, [(n, 1) for n in (1, 32, 63, 64, 65, 128, 129, 300)], 0),
+    ("the same, e4m3, 128 wide", 28, 4, 128, 16, True, [(n, 1) for n in (2, 47, 64, 130, 257)], 0),
+    ("one head per kv head", 3, 3, 128, 128, False, [(40, 1), (400, 1)], 0),
+    ("sixteen heads per kv head", 16, 1, 64, 256, False, [(40, 1), (700, 1)], 0),
+    ("forty heads per kv head", 40, 1, 64, 16, False, [(33, 1), (150, 2)], 0),
+    ("a long one and its split", 4, 2, 128, 16, False, [(5000, 1)], 0),
+    ("long and short", 6, 2, 64, 32, False, [(3000, 1), (1, 1), (7, 1), (2500, 1)], 0),
+    ("a few new tokens", 7, 1, 64, 16, False, [(200, 5), (5, 5), (64, 3), (65, 4), (1000, 2)], 0),
+    ("a few new tokens, e4m3", 8, 2, 128, 64, True, [(200, 5), (5, 5), (64, 3), (700, 8)], 0),
+    ("a short prompt", 14, 2, 64, 16, False, [(40, 40)], 0),
+    ("a prompt", 14, 2, 64, 64, False, [(333, 333)], 0),
+    ("a piece of a prompt", 8, 2, 128, 32, False, [(900, 131)], 0),
+    ("a piece of a prompt, e4m3", 4, 2, 128, 16, True, [(515, 150)], 0),
+    ("a piece of a prompt, e4m3, 64 wide", 6, 2, 64, 16, True, [(515, 150)], 0),
+    ("pieces beside tokens", 8, 2, 64, 16, False, [(300, 100), (50, 1), (129, 1), (64, 64), (700, 1)], 0),
+    ("pieces beside tokens, 128 wide", 6, 2, 128, 64, True, [(300, 100), (50, 1), (129, 1), (64, 64), (700, 1)], 0),
+    ("window of one", 4, 2, 64, 16, False, [(100, 1), (30, 30)], 1),
+    ("window inside a tile", 4, 2, 64, 16, False, [(100, 1), (300, 90), (20, 20)], 37),
+    ("window over tiles", 8, 1, 128, 32, False, [(700, 1), (600, 100), (99, 20)], 200),
+    ("window longer than the context", 4, 2, 64, 16, False, [(100, 1), (70, 40)], 1000),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=[c[0] for c in CASES])
+def test_attention(hk_lib, case):
+    name, hq, hkv, dim, page, e4m3, entries, window = case
+    announce(f"paged attention: {name}")
+    rng = np.random.default_rng(sum(map(ord, name)))
+    need = sum(-(-n // page) for n, _ in entries)
+    cache = Cache(rng, pages=need + 3, kv_heads=hkv, page=page, dim=dim, seqs=len(entries) + 2,
+                  width=max(-(-n // page) for n, _ in entries) + 1, e4m3=e4m3, gap=64)
+    cache.give([n for n, _ in entries], rng)
+    cache.fill(rng)
+    cache.upload()
+    seqs = list(range(len(entries)))
+    # the first two rows and the last one are of no entry
+    first = np.cumsum([2] + [c for _, c in entries])
+    q = _bits(rng.normal(size=(first[-1] + 1, hq, dim)) * 1.5)
+    scale = dim**-0.5
+    got, lse, raw = attention(cache, 0, q, seqs, first, scale=scale, window=window, stride=hq * dim + 24)
+    want = oracle.attention(cache.o, 0, _floats(q), seqs, first, scale, window)
+    check_attention(got, lse, raw, want, _floats(q), cache, scale)
+    # the same result whatever the caller says of the entries' rows, and once more from the same workspace
+    again = attention(cache, 0, q, seqs, first, scale=scale, window=window, stride=hq * dim + 24, want_lse=False)
+    np.testing.assert_array_equal(again[2], raw)
+    for max_new in (1, 4, 1000):
+        check_attention(*attention(cache, 0, q, seqs, first, scale=scale, window=window, max_new=max_new), want,
+                        _floats(q), cache, scale)
+
+
+def test_attention_of_odd_batches(hk_lib):
+    """Entries without rows, of length 0, longer than their sequence, of no sequence, with missing pages; the same
+    sequence in two entries; sequences in another order."""
+    announce("paged attention: odd batches")
+    rng = np.random.default_rng(5)
+    cache = Cache(rng, pages=40, kv_heads=2, page=16, dim=64, seqs=7, width=9)
+    cache.give([0, 3, 100, 130, 64, 50, 20], rng)
+    cache.fill(rng)
+    # missing: a page in the middle, the only page, ids past the pool
+    cache.o["table"][3, 2] = -1
+    cache.o["table"][6, :2] = (-7, 40)
+    cache.o["table"][5, 1] = 1 << 30
+    cache.upload()
+    seqs = [3, 0, 1, -1, 7, 6, 2, 2, 5, 4, 1 << 30]
+    counts = [20, 2, 5, 1, 3, 4, 1, 90, 3, 0, 2]
+    first = np.cumsum([0] + counts)
+    q = _bits(rng.normal(size=(first[-1] + 3, 6, 64)))
+    for window in (0, 18, 40):
+        for max_new in (None, 1):
+            got = attention(cache, 0, q, seqs, first, scale=0.2, window=window, max_new=max_new)
+            check_attention(*got, oracle.attention(cache.o, 0, _floats(q), seqs, first, 0.2, window), _floats(q),
+                            cache, 0.2)
+    # lengths and first rows beyond what there is
+    cache.o["length"][:] = (-5, 3, 10**9, 130, 64, 50, 20)
+    cache.o["table"][2, 7:] = -1
+    cache.upload()
+    first[-1] = 10**6
+    first[0] = -3
+    got = attention(cache, 0, q, seqs, first, scale=0.2, max_new=100)
+    check_attention(*got, oracle.attention(cache.o, 0, _floats(q), seqs, first, 0.2), _floats(q), cache, 0.2)
+
+
+@pytest.mark.parametrize("dim,e4m3,counts", [(64, False, (1, 1)), (64, False, (4, 7)), (128, False, (90, 70)),
+                                             (128, True, (90, 1)), (64, True, (3, 130))])
+def test_attention_ignores_what_a_row_does_not_see(hk_lib, dim, e4m3, counts):
+    """NaN and infinities in keys and values of later tokens, of slots left of the window, and behind the last slot."""
+    announce(f"paged attention: poisoned slots, dim {dim}, e4m3 {e4m3}, rows {counts}")
+    rng = np.random.default_rng(7)
+    cache = Cache(rng, pages=30, kv_heads=1, page=32, dim=dim, seqs=2, width=8, e4m3=e4m3)
+    cache.give([200, 147], rng)
+    cache.fill(rng)
+    bad = [np.nan] if e4m3 else [np.nan, np.inf, -np.inf]
+    window = 60
+    for s, c in enumerate(counts):
+        n = cache.o["length"][s]
+        spots = [n - c - window, 0]  # left of every row's window
+        if c > 1:
+            spots.append(n - 1)  # seen by the last row alone
+        for i, j in enumerate(spots):
+            page, at = cache.o["table"][s, j // 32], j % 32
+            cache.o["k"][0, page, 0, at, i] = bad[i % len(bad)]
+            cache.o["v"][0, page, 0, at, 3 + i] = bad[(i + 1) % len(bad)]
+    cache.upload()
+    first = np.cumsum([0] + list(counts))
+    q = _bits(rng.normal(size=(first[-1], 5, dim)))
+    got, lse, raw = attention(cache, 0, q, [0, 1], first, scale=0.1, window=window)
+    last = [first[i + 1] - 1 for i in range(2) if counts[i] > 1]
+    with np.errstate(invalid="ignore"):
+        want = oracle.attention(cache.o, 0, _floats(q), [0, 1], first, 0.1, window)
+    keep = np.ones(first[-1], bool)
+    keep[last] = False
+    for r in last:  # the rows that see the values show it
+        assert np.any(np.isnan(want[0][r]))
+        np.testing.assert_array_equal(np.isnan(got[r]), np.isnan(want[0][r]))
+    check_attention(got[keep], lse[keep], raw[keep], tuple(w[keep] for w in want), _floats(q)[keep], cache, 0.1)
+
+
+def test_attention_layers_and_far_pages(hk_lib):
+    """Layers of their own, and pages more than 4 GiB into the pool."""
+    from runtime import hip
+
+    announce("paged attention: pages beyond 32-bit offsets")
+    rng = np.random.default_rng(8)
+    cache = Cache(rng, layers=2, pages=6, kv_heads=1, page=16, dim=64, seqs=1, width=4, poison=False)
+    cache.give([50], rng)
+    for layer in (0, 1):
+        cache.fill(rng, layer)
+    cache.upload()
+    q = _bits(rng.normal(size=(2, 2, 64)))
+    for layer in (0, 1):
+        got = attention(cache, layer, q, [0], [0, 2], scale=0.125)
+        check_attention(*got, oracle.attention(cache.o, layer, _floats(q), [0], [0, 2], 0.125), _floats(q), cache,
+                        0.125)
+    # the same pages 1 GiB of elements apart: page 5 starts 10 GiB into a pool
+    stride = 1 << 30
+    far = {x: hip.DeviceBuffer(2 * (5 * stride + 16 * 64)) for x in "kv"}
+    for x in "kv":
+        rows = cache.encode(cache.o[x][1], x, 1)
+        for p in range(6):
+            far[x].write(rows[p], 2 * p * stride)
+        setattr(cache.c, x, far[x].ptr)
+    cache.c.page_stride, cache.c.layer_stride, cache.c.layers = stride, 6 * stride, 1
+    got = attention(cache, 0, q, [0], [0, 2], scale=0.125)
+    check_attention(*got, oracle.attention(cache.o, 1, _floats(q), [0], [0, 2], 0.125), _floats(q), cache, 0.125)
+
+
+# ---- append ----
+
+
+def _tables(slots, dim, rng):
+    angle = np.arange(slots)[:, None] * 10000.0 ** (-np.arange(dim // 2) / (dim // 2))
+    return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,page,e4m3,rope", [(14, 2, 64, 16, False, True), (9, 3, 64, 32, True, True),
+                                                       (8, 2, 128, 16, False, False), (28, 4, 128, 64, True, True)])
+def test_append(hk_lib, hq, hkv, dim, page, e4m3, rope):
+    """bf16: the numbers are one rounding of float32 a cos - b sin (half a step, 2^-8 relative to the result, after
+    products and a difference each rounded by 2^-24 of their operands); values are stored as they are.  e4m3: the
+    nearest code of x / scale, or its neighbour where float32 falls on the other side of a border."""
+    from runtime import hip, paged
+
+    announce(f"paged append: {hq}/{hkv} heads of {dim}, page {page}, e4m3 {e4m3}")
+    rng = np.random.default_rng(dim + page)
+    # a new sequence, one token, over a page's end, no rows, more rows than tokens, of no sequence
+    entries = [(0, 37, 37), (1, 50, 1), (2, page + 3, 9), (3, 20, 0), (4, 2, 5), (9, 0, 2)]
+    cache = Cache(rng, layers=2, pages=30, kv_heads=hkv, page=page, dim=dim, seqs=5, width=6, e4m3=e4m3, gap=32)
+    cache.give([n for _, n, _ in entries[:5]], rng)
+    for layer in (0, 1):
+        cache.fill(rng, layer)
+    cache.o["table"][2, 1] = -1  # where some of the rows would go
+    cache.upload()
+    untouched = [[cache.download(x, l).copy() for x in "kv"] for l in (0, 1)]
+    first = np.cumsum([1] + [c for _, _, c in entries])
+    tokens, stride = int(first[-1]) + 2, (hq + 2 * hkv) * dim + 16
+    qkv = np.full((tokens, stride), 0x7FC0, np.uint16)
+    x = _bits(rng.normal(size=(tokens, hq + 2 * hkv, dim)) * 3)
+    qkv[:, :-16] = x.reshape(tokens, -1)
+    if e4m3:  # saturation, and NaN which stays one
+        x[first[1], hq, 5] = _bits([1e6])[0]
+        x[first[1], hq + hkv, 6] = _bits([-1e6])[0]
+        x[first[1], hq + hkv, 7] = 0x7FC0
+        qkv[:, :-16] = x.reshape(tokens, -1)
+    cos, sin = _tables(6 * page, dim, rng) if rope else (None, None)
+    C, S = (None if t is None else _dev(t) for t in (cos, sin))
+    IN, OUT = _dev(qkv), _dev(np.full((tokens, hq * dim + 8), 0x4242, np.uint16))
+    SEQ, FIRST = _dev(np.array([s for s, _, _ in entries], np.int32)), _dev(first.astype(np.int32))
+
+    def call(q_out, q_stride):
+        hip.check(paged.lib().hk_paged_append(
+            ctypes.byref(cache.c), 1, IN.ptr, stride, C and C.ptr, S and S.ptr, 6 * page, SEQ.ptr, FIRST.ptr, len(entries),
+            tokens, hq, q_out, q_stride, None), "hk_paged_append")
+        _sync()
+
+    call(OUT.ptr, hq * dim + 8)
+    before = {y: cache.o[y].copy() for y in "kv"}
+    want = oracle.append(cache.o, 1, _floats(x), [s for s, _, _ in entries], first, hq, cos, sin, cache.store(1))
+    raw = OUT.read(np.uint16, tokens * (hq * dim + 8)).reshape(tokens, -1)
+    assert np.all(raw[:, hq * dim:] == 0x4242)
+    raw = raw[:, :hq * dim].reshape(tokens, hq, dim)
+    mine = ~np.isnan(want[:, 0, 0])
+    assert np.all(raw[~mine] == 0x4242)
+    f = np.abs(_floats(x)[:, :hq])
+    a = f + np.roll(f, dim // 2, -1)
+    assert np.all(np.abs(_floats(raw)[mine] - want[mine]) <= 2.0**-8 * np.abs(want[mine]) + 2.0**-23 * a[mine])
+    for y, i in (("k", 0), ("v", 1)):
+        got = cache.download(y, 1)
+        written = ~((cache.o[y][1] == before[y][1]) | (np.isnan(cache.o[y][1]) & np.isnan(before[y][1])))
+        np.testing.assert_array_equal(got[~written], untouched[1][i][~written])
+        want_codes = cache.encode(cache.o[y][1], y, 1)
+        step = np.abs(got[written].astype(int) - want_codes[written].astype(int))
+        if e4m3:  # (a NaN's sign says nothing)
+            step[(got[written] & 0x7F == 0x7F) & (want_codes[written] == 0x7F)] = 0
+        assert step.max() <= 1 and (step == 0).mean() > 0.99 and (y == "k" or step.max() == 0)
+        np.testing.assert_array_equal(cache.download(y, 0), untouched[0][i])
+    # in place, and without queries
+    call(IN.ptr, stride)
+    back = IN.read(np.uint16, tokens * stride).reshape(tokens, stride)
+    np.testing.assert_array_equal(back[:, :hq * dim].reshape(raw.shape)[mine], raw[mine])
+    np.testing.assert_array_equal(back[:, hq * dim:], qkv[:, hq * dim:])
+    once = [cache.download(y, 1) for y in "kv"]
+    call(None, 0)
+    for y, was in zip("kv", once):
+        np.testing.assert_array_equal(cache.download(y, 1), was)
+
+
+def test_append_is_the_decode_steps_append(hk_lib):
+    """The rows that hk_attention_decode puts into its contiguous cache, bit for bit, and its attention's numbers."""
+    from runtime import hip
+    from runtime.qwen_engine import rope_tables
+
+    announce("paged append and attention against hk_attention_decode")
+    rng = np.random.default_rng(11)
+    hq, hkv, ctx, p = 14, 2, 512, 300
+    cos, sin = rope_tables(1e6, 64, ctx)
+    kc, vc = (np.zeros((hkv, ctx, 64), np.uint16) for _ in range(2))
+    kc[:, :p], vc[:, :p] = (_bits(rng.normal(size=(hkv, p, 64))) for _ in range(2))
+    qkv = _bits(rng.normal(size=(hq + 2 * hkv) * 64))
+    QKV, COS, SIN, KC, VC = map(_dev, (qkv, cos, sin, kc, vc))
+    OUT = hip.DeviceBuffer(2 * hq * 64)
+    hip.check(hk_lib.hk_attention_decode(QKV.ptr, COS.ptr, SIN.ptr, KC.ptr, VC.ptr, p, ctx, hq, hkv, 64, OUT.ptr, None),
+              "hk_attention_decode")
+    _sync()
+    want = OUT.read(np.uint16, hq * 64)
+    from runtime import paged
+
+    cache = Cache(rng, pages=40, kv_heads=hkv, page=16, dim=64, seqs=1, width=32)
+    cache.give([p + 1], rng)
+    slot, page, at = oracle.slots_of(cache.o, 0, p)
+    for x, rows in (("k", kc), ("v", vc)):
+        cache.o[x][0, page, :, at] = _floats(rows[:, :p]).transpose(1, 0, 2)
+    cache.upload()
+    SEQ, FIRST, Q = _dev(np.zeros(1, np.int32)), _dev(np.array([0, 1], np.int32)), hip.DeviceBuffer(2 * hq * 64)
+    hip.check(paged.lib().hk_paged_append(ctypes.byref(cache.c), 0, QKV.ptr, (hq + 2 * hkv) * 64, COS.ptr, SIN.ptr, ctx,
+                                          None, FIRST.ptr, 1, 1, hq, Q.ptr, hq * 64, None), "hk_paged_append")
+    _sync()
+    for x, ref in (("k", KC), ("v", VC)):
+        held = ref.read(np.uint16, hkv * ctx * 64).reshape(hkv, ctx, 64)[:, p]
+        np.testing.assert_array_equal(cache.download(x, 0)[cache.o["table"][0, p // 16], :, p % 16], held)
+        cache.o[x][0, cache.o["table"][0, p // 16], :, p % 16] = _floats(held)
+    q = Q.read(np.uint16, hq * 64).reshape(1, hq, 64)
+    got = attention(cache, 0, q, [0], [0, 1], scale=0.125)
+    ref = oracle.attention(cache.o, 0, _floats(q), [0], [0, 1], 0.125)
+    check_attention(*got, ref, _floats(q), cache, 0.125)
+    # both within their tolerance of float64: a bf16 step of each other and the probabilities' rounding
+    assert np.all(np.abs(_floats(want).reshape(1, hq, 64) - got[0]) <= 2.0**-7 * np.abs(ref[0]) + 2.0**-8 * ref[2] * 1.1)
+
+
+# ---- fork and compaction ----
+
+
+def fork(cache, child, parent, keep, grow):
+    """Both forks; the status words."""
+    from runtime import hip, paged
+
+    arrays = [None if a is None else _dev(np.asarray(a, np.int32)) for a in (child, parent, keep, grow)]
+    S = _dev(np.full(2, -9, np.int32))
+    n = len(next(a for a in (child, parent, keep, grow) if a is not None))
+    hip.check(paged.lib().hk_paged_fork(ctypes.byref(cache.c), *(a and a.ptr for a in arrays), n, S.ptr,
+                                        cache.bufs["workspace"].ptr, None), "hk_paged_fork")
+    _sync()
+    return tuple(S.read(np.int32, 2).tolist())
+
+
+def same(cache):
+    """The GPU's cache is the oracle's, all of it."""
+    for x in ("table", "length", "refs"):
+        np.testing.assert_array_equal(cache.bufs[x].read(np.int32, cache.o[x].size).reshape(cache.o[x].shape), cache.o[x],
+                                      err_msg=x)
+    for l in range(cache.o["k"].shape[0]):
+        for x in "kv":
+            np.testing.assert_array_equal(cache.download(x, l), cache.encode(cache.o[x][l], x, l), err_msg=x)
+
+
+@pytest.mark.parametrize("page,dim,e4m3,seed", [(16, 64, False, 0), (32, 128, True, 1), (64, 64, True, 2)])
+def test_fork_and_compact_in_random_order(hk_lib, page, dim, e4m3, seed):
+    """A hundred random calls: new answers, reordered beams, tokens added and taken back, sequences freed, entries
+    that are not valid, pools too full, compactions, each compared with the oracle's whole cache."""
+    from runtime import hip, paged
+
+    announce(f"paged fork: page {page}, dim {dim}, e4m3 {e4m3}")
+    rng = np.random.default_rng(seed)
+    seqs, width = 9, 6
+    cache = Cache(rng, layers=2, pages=10, kv_heads=2, page=page, dim=dim, seqs=seqs, width=width, e4m3=e4m3, gap=16,
+                  poison=False)
+    outcomes = set()
+    for step in range(100):
+        n = int(rng.integers(1, seqs + 1))
+        child = rng.permutation(seqs)[:n]
+        kind = rng.integers(0, 6)
+        length = cache.o["length"]
+        if kind == 0:  # the next tokens
+            parent, keep, grow = child, length[child], rng.integers(0, page, n)
+        elif kind == 1:  # answers and beams
+            parent = rng.integers(0, seqs, n)
+            keep, grow = length[parent], rng.integers(0, 3, n)
+        elif kind == 2:  # prefixes
+            parent = rng.integers(0, seqs, n)
+            keep, grow = rng.integers(0, length[parent] + 1), rng.integers(0, page, n)
+        elif kind == 3:  # freeing
+            parent, keep, grow = np.full(n, -1), np.zeros(n, int), np.zeros(n, int)
+        elif kind == 4 and step % 3 == 0:  # not valid in one of several ways
+            parent, keep, grow = child.copy(), length[child].copy(), np.ones(n, int)
+            i = int(rng.integers(n))
+            bad = rng.integers(0, 6)
+            if bad == 0 and n > 1:
+                child[i] = child[i - 1]
+            elif bad == 1:
+                child[i] = seqs
+            elif bad == 2:
+                keep[i] += 1
+            elif bad == 3:
+                parent[i], keep[i] = -1, 1
+            elif bad == 4:
+                grow[i] = width * page
+            else:
+                grow[i] = -1
+        else:
+            live = oracle.compact(cache.o)
+            L = _dev(np.zeros(1, np.int32))
+            hip.check(paged.lib().hk_paged_compact(ctypes.byref(cache.c), cache.c.table, cache.c.refs, L.ptr,
+                                                   cache.bufs["workspace"].ptr, None), "hk_paged_compact")
+            _sync()
+            assert L.read(np.int32, 1)[0] == live
+            same(cache)
+            continue
+        want = oracle.fork(cache.o, *(list(map(int, a)) for a in (child, parent, keep, grow)))
+        assert fork(cache, child, parent, keep, grow) == want, (step, kind)
+        outcomes.add(want[0])
+        same(cache)
+        if want[0] == 0 and rng.random() < 0.5:  # contents that tell the pages apart
+            cache.fill(rng, int(rng.integers(2)))
+            cache.upload()
+    assert outcomes == {0, 1, 2}
+
+
+def test_fork_defaults_and_aliases(hk_lib):
+    """NULL arrays, and `keep` that is the cache's own lengths."""
+    from runtime import hip, paged
+
+    announce("paged fork: defaults")
+    rng = np.random.default_rng(3)
+    cache = Cache(rng, pages=12, kv_heads=1, page=16, dim=64, seqs=3, width=4, poison=False)
+    cache.give([5, 16, 31], rng)
+    cache.fill(rng)
+    cache.upload()
+    S, G = _dev(np.zeros(2, np.int32)), _dev(np.array([1, 1, 2], np.int32))
+    for grow, keep in ((None, None), (G.ptr, None), (G.ptr, cache.c.length), (cache.c.length, cache.c.length)):
+        hip.check(paged.lib().hk_paged_fork(ctypes.byref(cache.c), None, None, keep, grow, 3, S.ptr,
+                                            cache.bufs["workspace"].ptr, None), "hk_paged_fork")
+        _sync()
+        n = cache.o["length"].tolist()
+        add = [0] * 3 if grow is None else [1, 1, 2] if grow == G.ptr else n
+        assert tuple(S.read(np.int32, 2)) == oracle.fork(cache.o, [0, 1, 2], [0, 1, 2], n, add)
+        same(cache)
+
+
+@pytest.mark.parametrize("pages,seqs", [(1, 1), (64, 5), (1500, 130), (5000, 1030)])
+def test_fork_and_compact_sizes(hk_lib, pages, seqs):
+    """Pools of more pages, and calls of more entries, than a workgroup has threads; compaction into other tables."""
+    from runtime import hip, paged
+
+    announce(f"paged fork: {pages} pages, {seqs} sequences")
+    rng = np.random.default_rng(pages)
+    width = max(1, pages // seqs - 1)
+    cache = Cache(rng, pages=pages, kv_heads=1, page=16, dim=64, seqs=seqs, width=width, poison=False)
+    grow = rng.integers(0, 16 * width + 1, seqs)
+    zero = [0] * seqs
+    assert fork(cache, None, None, zero, grow) == oracle.fork(cache.o, range(seqs), range(seqs), zero, grow) == (0, 0)
+    cache.fill(rng)
+    cache.upload()
+    child = rng.permutation(seqs)
+    parent = rng.integers(0, seqs, seqs)
+    keep = [int(rng.integers(0, cache.o["length"][p] + 1)) for p in parent]
+    assert fork(cache, child, parent, keep, zero) == oracle.fork(cache.o, child, parent, keep, zero) == (0, 0)
+    same(cache)
+    T, R, L = _dev(np.zeros_like(cache.o["table"])), _dev(np.zeros_like(cache.o["refs"])), _dev(np.zeros(1, np.int32))
+    was = {x: cache.o[x].copy() for x in ("table", "refs")}
+    hip.check(paged.lib().hk_paged_compact(ctypes.byref(cache.c), T.ptr, R.ptr, L.ptr, cache.bufs["workspace"].ptr, None),
+              "hk_paged_compact")
+    _sync()
+    assert oracle.compact(cache.o) == L.read(np.int32, 1)[0]
+    np.testing.assert_array_equal(T.read(np.int32, cache.o["table"].size), cache.o["table"].ravel())
+    np.testing.assert_array_equal(R.read(np.int32, pages), cache.o["refs"])
+    cache.o.update(was)
+    same(cache)
+
+
+# ---- together ----
+
+
+def test_chats_share_a_prompt(hk_lib):
+    """As a server uses it: a prompt in two pieces, three answers forked from it, decode steps of all of them at once
+    over two layers, one taken back, one freed, the pool compacted, and on.  Each attention against the oracle."""
+    from runtime import paged
+
+    announce("paged cache: chats that share a prompt")
+    rng = np.random.default_rng(21)
+    hq, hkv, dim, page, layers = 6, 2, 64, 16, 2
+    kv = paged.PagedKV(layers=layers, kv_heads=hkv, head_dim=dim, page_size=page, pages=30, seqs=5, table_width=8)
+    cos, sin = _tables(8 * page, dim, rng)
+    C, S = _dev(cos), _dev(sin)
+    o = {"k": np.zeros((layers, 30, hkv, page, dim)), "v": np.zeros((layers, 30, hkv, page, dim)),
+         "table": np.full((5, 8), -1, np.int32), "length": np.zeros(5, np.int32), "refs": np.zeros(30, np.int32)}
+
+    def forked(child, parent, keep, grow):
+        assert oracle.fork(o, child, parent, keep, grow) == (0, 0)
+        kv.fork(child, parent, keep, grow)
+        for name in ("table", "length", "refs"):
+            got = {"table": kv.table, "length": kv.lengths, "refs": kv.refs}[name]()
+            np.testing.assert_array_equal(got, o[name])
+
+    def stepped(seqs, counts):
+        first = np.cumsum([0] + counts)
+        for layer in range(layers):
+            x = _bits(rng.normal(size=(first[-1], hq + 2 * hkv, dim)))
+            IN, Q, OUT = _dev(x), _dev(np.zeros((first[-1], hq, dim), np.uint16)), _dev(np.zeros((first[-1], hq, dim),
+                                                                                               np.uint16))
+            kv.append(layer, IN.ptr, seqs, first, hq, rope=(C.ptr, S.ptr, 8 * page), q_out=Q.ptr)
+            kv.attention(layer, Q.ptr, seqs, first, hq, OUT.ptr)
+            _sync()
+            oracle.append(o, layer, _floats(x), seqs, first, hq, cos, sin, lambda rows, which: _floats(_bits(rows)))
+            q = _floats(Q.read(np.uint16, Q.nbytes // 2).reshape(-1, hq, dim))
+            got = _floats(OUT.read(np.uint16, OUT.nbytes // 2).reshape(-1, hq, dim))
+            want, _, spread = oracle.attention(o, layer, q, seqs, first, dim**-0.5)
+            # the keys' float32 rotation may round to the neighbouring bf16: 2^-8 |k_d| at every dimension, so a score
+            # by up to 2^-8 scale sum |q_d k_d|, a few per cent of the keys; then the tolerances of the top
+            tol = 2.0**-8 * np.abs(want) + (2.0**-8 + 2.0**-8) * spread + 1e-30
+            assert np.all(np.abs(got - want) <= tol)
+
+    forked([0], [0], [0], [21])
+    stepped([0], [21])
+    forked([0], [0], [21], [30])
+    stepped([0], [30])
+    forked([1, 2, 3], [0, 0, 0], [51, 51, 40], [1, 1, 2])
+    stepped([1, 2, 3], [1, 1, 2])
+    for _ in range(14):
+        n = [int(x) for x in o["length"]]
+        forked([0, 1, 2, 3], [0, 1, 2, 3], n[:4], [1] * 4)
+        stepped([2, 0, 1, 3], [1] * 4)
+    n = [int(x) for x in o["length"]]
+    forked([1, 2], [1, 2], [n[1] - 20, 0], [3, 0])  # taken back and corrected; freed
+    stepped([1], [3])
+    assert kv.compact() == oracle.compact(o)
+    np.testing.assert_array_equal(kv.table(), o["table"])
+    np.testing.assert_array_equal(kv.refs(), o["refs"])
+    for _ in range(3):
+        n = [int(x) for x in o["length"]]
+        forked([0, 1, 3], [0, 1, 3], [n[0], n[1], n[3]], [1, 2, 1])
+        stepped([0, 1, 3], [1, 2, 1])
+    kv.release([0, 1, 3])
+    assert np.all(kv.refs() == 0) and np.all(kv.lengths() == 0)
+    with pytest.raises(ValueError):
+        kv.fork([0], [1], [5], [0])
+    with pytest.raises(RuntimeError):
+        kv.fork([0, 1, 2, 3], [0] * 4, [0] * 4, [8 * page] * 4)
+    kv.close()

@@ -1,0 +1,219 @@
+"""The paged cache without a GPU: the exports and binding of include/hk_paged.h, what the calls refuse before any
+device work, and the float64 oracle against other formulations."""
+
+import ctypes
+import re
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+from oracle import paged as oracle
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def test_exports_and_binding():
+    from runtime import hip, paged
+
+    text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "hk_paged.h").read_text(), flags=re.S)
+    names = set(re.findall(r"\b(hk_paged_[a-z0-9_]+)\s*\(", text))
+    assert names == set(paged.EXPORTED) == {"hk_paged_append", "hk_paged_attention", "hk_paged_fork",
+                                            "hk_paged_compact"}
+    lib = ctypes.CDLL(str(hip.LIB_PATH))
+    assert all(hasattr(lib, n) for n in names)
+    assert int(re.search(r"HK_PAGED_WORKSPACE (\d+)", text).group(1)) == paged.WORKSPACE
+    fields = re.search(r"typedef struct hk_paged_cache \{(.*?)\}", text, flags=re.S).group(1)
+    assert re.findall(r"(\w+);", fields) == [n for n, _ in paged.PagedCache._fields_]
+
+
+# Host memory stands in for device pointers: a refused call never looks at it.
+HERE = (ctypes.c_char * 4096)()
+AT = -(-ctypes.addressof(HERE) // 256) * 256
+
+
+def _cache(**changes):
+    from runtime import paged
+
+    c = dict(k=AT, v=AT, k_scale=None, v_scale=None, table=AT, length=AT, refs=AT, layer_stride=1 << 20,
+             page_stride=2 * 16 * 64, layers=2, kv_heads=2, head_dim=64, page_size=16, pages=8, seqs=4, table_width=4,
+             dtype=paged.BF16)
+    c.update(changes)
+    return paged.PagedCache(**c)
+
+
+APPEND = dict(layer=0, qkv=AT, qkv_stride=512, cos=AT, sin=AT, positions=64, seqs=AT, first=AT, n=2, tokens=3,
+              q_heads=4, q_out=AT + 1024, q_out_stride=256, stream=None)
+ATTENTION = dict(layer=0, q=AT, q_stride=256, seqs=AT, first=AT, n=2, tokens=3, max_new=2, q_heads=4, scale=0.125,
+                 window=0, out=AT, out_stride=256, lse=None, workspace=AT, stream=None)
+FORK = dict(child=None, parent=None, keep=None, grow=None, n=2, status=AT, workspace=AT, stream=None)
+COMPACT = dict(table_out=AT, refs_out=AT, live_out=AT, workspace=AT, stream=None)
+CALLS = {"hk_paged_append": APPEND, "hk_paged_attention": ATTENTION, "hk_paged_fork": FORK, "hk_paged_compact": COMPACT}
+
+
+def _refused(name, cache, rc, **changes):
+    from runtime import hip, paged
+
+    args = dict(CALLS[name], **changes)
+    got = getattr(paged.lib(), name)(None if cache is None else ctypes.byref(cache), *args.values())
+    assert got == rc, (got, hip.last_error())
+    assert hip.last_error().startswith(name)
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_refuses_bad_caches(name):
+    from runtime import hip, paged
+
+    bad, unsupported = hip.HK_ERR_INVALID, hip.HK_ERR_UNSUPPORTED
+    _refused(name, None, bad)
+    for field in ("k", "v", "table", "length", "refs"):
+        _refused(name, _cache(**{field: None}), bad)
+    for changes, rc in ((dict(head_dim=96), unsupported), (dict(page_size=8), unsupported),
+                        (dict(page_size=48), unsupported), (dict(page_size=512), unsupported), (dict(dtype=2), bad),
+                        (dict(layers=0), bad), (dict(kv_heads=0), bad), (dict(pages=0), bad), (dict(seqs=-1), bad),
+                        (dict(table_width=0), bad), (dict(table_width=1 << 27), bad),
+                        (dict(page_stride=2 * 16 * 64 - 8), bad), (dict(page_stride=2 * 16 * 64 + 4), bad),
+                        (dict(layer_stride=2 * 16 * 64 - 8), bad), (dict(layer_stride=2 * 16 * 64 + 1), bad),
+                        (dict(k=AT + 8), bad), (dict(v=AT + 2), bad), (dict(dtype=paged.E4M3), bad),
+                        (dict(dtype=paged.E4M3, k_scale=AT), bad),
+                        (dict(dtype=paged.E4M3, k_scale=AT, v_scale=AT, page_stride=2 * 16 * 64 + 8), bad)):
+        _refused(name, _cache(**changes), rc)
+
+
+@pytest.mark.parametrize("name", ["hk_paged_append", "hk_paged_attention"])
+def test_refuses_bad_batches(name):
+    from runtime import hip
+
+    for changes in (dict(layer=-1), dict(layer=2), dict(first=None), dict(n=-1), dict(tokens=-1), dict(n=4097),
+                    dict(q_heads=3), dict(q_heads=0), dict(q_heads=8192)):
+        _refused(name, _cache(), hip.HK_ERR_INVALID, **changes)
+
+
+def test_refuses_bad_arguments():
+    from runtime import hip, paged
+
+    bad = hip.HK_ERR_INVALID
+    for changes in (dict(qkv=None), dict(qkv=AT + 2), dict(qkv_stride=511), dict(qkv_stride=504), dict(q_out=AT + 8),
+                    dict(q_out_stride=248), dict(cos=None), dict(sin=None), dict(sin=AT + 4), dict(positions=63),
+                    dict(q_out_stride=256, q_out=APPEND["qkv"], qkv_stride=520)):
+        _refused("hk_paged_append", _cache(), bad, **changes)
+    for changes in (dict(q=None), dict(out=None), dict(q=AT + 8), dict(out=AT + 4), dict(q_stride=248),
+                    dict(out_stride=260), dict(workspace=None), dict(workspace=AT + 16), dict(max_new=0),
+                    dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                    dict(scale=float("inf"))):
+        _refused("hk_paged_attention", _cache(), bad, **changes)
+    for changes in (dict(status=None), dict(workspace=None), dict(workspace=AT + 8), dict(n=0), dict(n=5)):
+        _refused("hk_paged_fork", _cache(), bad, **changes)
+    _refused("hk_paged_fork", _cache(seqs=30000, table_width=1000), hip.HK_ERR_UNSUPPORTED, n=30000)
+    for changes in (dict(table_out=None), dict(refs_out=None), dict(live_out=None), dict(workspace=None)):
+        _refused("hk_paged_compact", _cache(), bad, **changes)
+    _refused("hk_paged_compact", _cache(pages=1 << 24), hip.HK_ERR_UNSUPPORTED)
+    # nothing to do is no error
+    for name in ("hk_paged_append", "hk_paged_attention"):
+        for changes in (dict(n=0), dict(tokens=0)):
+            args = dict(CALLS[name], **changes)
+            assert getattr(paged.lib(), name)(ctypes.byref(_cache()), *args.values()) == hip.HK_OK
+
+
+# ---- the oracle ----
+
+
+def test_oracle_e4m3_rounds_to_nearest_even():
+    torch = pytest.importorskip("torch")
+    codes = np.arange(256, dtype=np.uint8)
+    want = torch.from_numpy(codes).view(torch.float8_e4m3fn).double().numpy()
+    np.testing.assert_array_equal(oracle.from_e4m3(codes), want)
+    rng = np.random.default_rng(0)
+    steps = oracle.from_e4m3(np.arange(127))
+    x = np.concatenate((rng.normal(0, 50, 4000), rng.normal(0, 0.01, 4000), (steps[1:] + steps[:-1]) / 2, steps, -steps,
+                        [448.0, 463.9, 0.0, -0.0]))
+    x = x.astype(np.float32)
+    got = torch.from_numpy(x).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    np.testing.assert_array_equal(oracle.e4m3(x), got)
+    assert oracle.e4m3(np.nan) == 0x7F and oracle.e4m3(np.inf) == 0x7E and oracle.e4m3(-1e9) == 0xFE
+
+
+def _random_cache(rng, layers=1, pages=12, heads=2, page=16, dim=64, seqs=4, width=6):
+    return {"k": rng.normal(size=(layers, pages, heads, page, dim)), "v": rng.normal(size=(layers, pages, heads, page, dim)),
+            "table": np.full((seqs, width), -1, np.int32), "length": np.zeros(seqs, np.int32),
+            "refs": np.zeros(pages, np.int32)}
+
+
+def test_oracle_attention_is_softmax_over_the_visible_slots():
+    rng = np.random.default_rng(1)
+    c = _random_cache(rng)
+    c["table"][0, :3], c["length"][0] = (7, 2, 9), 41
+    q = rng.normal(size=(5, 4, 64))
+    k = np.concatenate([c["k"][0, p] for p in (7, 2, 9)], 1)[:, :41]
+    v = np.concatenate([c["v"][0, p] for p in (7, 2, 9)], 1)[:, :41]
+    for window in (0, 1, 20):
+        out, lse, spread = oracle.attention(c, 0, q, [0], [0, 5], 0.3, window)
+        for t in range(5):
+            lo = max(0, 36 + t - window + 1) if window else 0
+            for h in range(4):
+                s = 0.3 * k[h // 2, lo:37 + t] @ q[t, h]
+                p = np.exp(s) / np.exp(s).sum()
+                np.testing.assert_allclose(out[t, h], p @ v[h // 2, lo:37 + t], rtol=1e-12, atol=1e-12)
+                np.testing.assert_allclose(lse[t, h], np.log(np.exp(s).sum()), rtol=1e-12)
+    # a planted mistake is caught: one slot more
+    assert np.abs(oracle.attention(c, 0, q, [0], [0, 4], 0.3)[0][:4] - out[:4]).max() > 1e-3
+    # rows before the first token, rows of no entry, an absent page
+    c["length"][0] = 2
+    out, lse, _ = oracle.attention(c, 0, q, [0, 9], [0, 4, 5], 1.0)
+    assert np.all(out[:2] == 0) and np.all(lse[:2] == -np.inf) and np.all(lse[4] == -np.inf)
+    np.testing.assert_array_equal(out[2, 0], v[0, 0])
+
+
+def _held(c):
+    """refs as the tables say."""
+    n = np.zeros(len(c["refs"]), np.int64)
+    for s, length in enumerate(c["length"]):
+        for p in c["table"][s, :-(-length // c["k"].shape[3])]:
+            n[p] += 1
+    return n
+
+
+def _tokens(c, s):
+    """What a sequence says: its key rows in order."""
+    page = c["k"].shape[3]
+    return np.concatenate([c["k"][:, p] for p in c["table"][s, :-(-c["length"][s] // page)]] or [c["k"][:, 0][:, :, :0]],
+                          2)[:, :, :c["length"][s]]
+
+
+def test_oracle_fork_keeps_contents_and_counts():
+    rng = np.random.default_rng(2)
+    c = _random_cache(rng, layers=2, pages=16)
+    free = lambda: int((c["refs"] == 0).sum())  # noqa: E731
+    assert oracle.fork(c, [0, 1], [0, 1], [0, 0], [37, 16]) == (0, 0)
+    assert c["length"].tolist() == [37, 16, 0, 0] and free() == 16 - 4
+    told = _tokens(c, 0)
+    assert oracle.fork(c, [2, 3, 0], [0, 0, 0], [37, 20, 37], [0, 1, 1]) == (0, 0)
+    # two full pages shared; 2 and 0 differ in the last page, 3 copied 4 slots of the second
+    assert c["refs"].tolist() == _held(c).tolist() and sorted(c["refs"])[-1] == 3
+    for s, n in ((0, 37), (2, 37), (3, 20)):
+        np.testing.assert_array_equal(_tokens(c, s)[:, :, :n], told[:, :, :n])
+    # beams reordered: everyone's parent is another child
+    before = [_tokens(c, s) for s in range(4)]
+    keep = c["length"].tolist()
+    assert oracle.fork(c, [0, 1, 2, 3], [1, 2, 3, 0], keep[1:] + keep[:1], [0] * 4) == (0, 0)
+    for s in range(4):
+        np.testing.assert_array_equal(_tokens(c, s), before[(s + 1) % 4])
+    assert c["refs"].tolist() == _held(c).tolist()
+    # what is not valid, and too little room, changes nothing
+    state = {x: c[x].copy() for x in c}
+    n = [int(x) for x in c["length"]]
+    for args, status in ((([0, 0], [0, 0], [0, 0], [0, 0]), (1, 1)), (([4], [0], [0], [0]), (1, 0)),
+                         (([0], [0], [n[0] + 1], [0]), (1, 0)), (([1, 0], [1, 9], [n[1], 1], [0, 0]), (1, 1)),
+                         (([0], [0], [n[0]], [96]), (1, 0)), (([0], [0], [-1], [0]), (1, 0))):
+        assert oracle.fork(c, *args) == status
+    code, missing = oracle.fork(c, [0, 1, 2, 3], [0, 1, 2, 3], n, [96 - x for x in n])
+    assert code == 2 and missing > 0
+    for x in state:
+        np.testing.assert_array_equal(c[x], state[x])
+    # compaction and freeing
+    told = [_tokens(c, s) for s in range(4)]
+    live = oracle.compact(c)
+    assert live == (c["refs"] > 0).sum() and np.all(c["refs"][:live] > 0)
+    for s in range(4):
+        np.testing.assert_array_equal(_tokens(c, s), told[s])
+    assert oracle.fork(c, [0, 1, 2, 3], [9] * 4, [0] * 4, [0] * 4) == (0, 0) and free() == 16
