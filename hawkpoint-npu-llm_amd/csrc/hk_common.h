@@ -142,6 +142,24 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
+// The maximum and the sum over lanes L, L ^ 16, L ^ 32, L ^ 48, the same value in each of the four: permlane32_swap of
+// two copies leaves lanes L and L ^ 32 in the two results, permlane16_swap
+// then lanes L and L ^ 16 (VALU lane swaps, where a shuffle goes through the
+// LDS).  The sum is (v_L + v_L^32) + (v_L^16 + v_L^48) in every lane.
+__device__ __forceinline__ float quad_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float quad_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 __device__ __forceinline__ uint64_t umax64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {

@@ -1198,25 +1198,6 @@ constexpr int kFaStreams = 2;               // KV streams per workgroup for 128-
 // units so that each exponential is one v_exp_f32
 constexpr float kFaScale = 0.125f * 1.4426950408889634f;
 
-// The maximum and the sum over lanes L, L ^ 16, L ^ 32, L ^ 48 (a token's
-// four lane groups), the same value in each of the four: permlane32_swap of
-// two copies leaves lanes L and L ^ 32 in the two results, permlane16_swap
-// then lanes L and L ^ 16 (VALU lane swaps, where a shuffle goes through the
-// LDS).  The sum is (v_L + v_L^32) + (v_L^16 + v_L^48) in every lane.
-__device__ __forceinline__ float quad_max(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-__device__ __forceinline__ float quad_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // KS: KV slots per block, kFaSlots, or 64 when the whole context fits 64
 // slots (a short prompt from slot 0: half the products of a 128-slot block,
 // whose second half is masked; the masked slots add exact zeros, so both

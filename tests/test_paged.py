@@ -3,6 +3,7 @@ device work, and the float64 oracle against other formulations."""
 
 import ctypes
 import re
+import subprocess
 from pathlib import Path
 
 import numpy as np
@@ -217,3 +218,99 @@ def test_oracle_fork_keeps_contents_and_counts():
     for s in range(4):
         np.testing.assert_array_equal(_tokens(c, s), told[s])
     assert oracle.fork(c, [0, 1, 2, 3], [9] * 4, [0] * 4, [0] * 4) == (0, 0) and free() == 16
+
+
+# ---- the cut of the attention's work ----
+
+PLAN = """
+#include "paged_plan.h"
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <set>
+#include <tuple>
+#include <vector>
+using namespace hk;
+#define CHECK(x) if (!(x)) { std::printf("%s, seed %d\\n", #x, seed); return 1; }
+int main() {
+  for (int seed = 0; seed < 400; ++seed) {
+    std::mt19937 rng(seed);
+    auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+    const int rows[] = {16, 32, 64, 256}, slots[] = {64, 128};
+    PlanShape s{pick(1, 4), pick(1, 9), pick(0, 2) ? 0 : pick(1, 300), rows[pick(0, 3)], slots[pick(0, 1)]};
+    std::vector<PlanEntry> e(pick(1, 12));
+    for (auto& x : e) x = {pick(0, 3) ? pick(0, 2000) : 0, pick(0, 3) ? pick(0, 3) : pick(0, 700)};
+    int64_t total = 0;
+    std::vector<int64_t> start;
+    for (auto& x : e) start.push_back(total), total += s.heads * plan_head_units(s, x);
+    const int groups = pick(1, 40);
+    const int64_t per = plan_per(total, groups, pick(1, 4));
+    std::map<std::tuple<int, int, int>, std::vector<int>> got;  // task: units
+    std::map<std::tuple<int, int, int>, int> arrived, asked, ticket;
+    std::set<int> partials;
+    for (int w = 0; w < groups; ++w) {
+      int64_t u = w * per;
+      const int64_t end = std::min(total, u + per);
+      if (u >= end) continue;
+      size_t i = 0;
+      while (i + 1 < e.size() && start[i + 1] <= u) ++i;
+      PlanPlace p = plan_find(s, e[i], (int)i, start[i], u - start[i]);
+      while (u < end) {
+        const PlanSpan span = plan_span(s, e[p.entry], p.tile);
+        const int units = plan_units(span), take = (int)std::min<int64_t>(units - p.at, end - u);
+        const auto task = std::make_tuple(p.entry, p.head, p.tile);
+        CHECK(p.start + p.at == u && take > 0);
+        for (int k = 0; k < take; ++k) got[task].push_back(p.at + k);
+        if (take < units) {
+          const PlanParts parts = plan_parts(p.start, units, per);
+          const int slot = plan_slot(p.start, w, per);
+          CHECK(w >= parts.first && w < parts.first + parts.count && parts.count > 1);
+          CHECK(partials.insert(slot).second && slot < 2 * groups);
+          CHECK(!ticket.count(task) || ticket[task] == parts.first);
+          ticket[task] = parts.first, asked[task] = parts.count, ++arrived[task];
+        }
+        u += take;
+        p.at = 0, p.start += units;
+        if (++p.tile >= plan_tiles(s, e[p.entry])) {
+          p.tile = 0;
+          if (++p.head >= s.heads) {
+            p.head = 0, ++p.entry;
+            while (p.entry < (int)e.size() && e[p.entry].count == 0) ++p.entry;
+          }
+        }
+      }
+    }
+    std::set<int> tickets;
+    for (auto& t : ticket) CHECK(tickets.insert(t.second).second && asked[t.first] == arrived[t.first]);
+    // every task once, its units in order; every slot that a row sees inside a block of its tile
+    size_t tasks = 0;
+    for (size_t i = 0; i < e.size(); ++i)
+      for (int t = 0; t < plan_tiles(s, e[i]); ++t) {
+        const PlanSpan span = plan_span(s, e[i], t);
+        tasks += s.heads;
+        for (int h = 0; h < s.heads; ++h) {
+          const auto& units = got[std::make_tuple((int)i, h, t)];
+          CHECK((int)units.size() == plan_units(span));
+          for (size_t k = 0; k < units.size(); ++k) CHECK(units[k] == (int)k);
+        }
+        for (int r = t * s.rows; r < std::min((t + 1) * s.rows, e[i].count * s.group); ++r) {
+          const int p = e[i].length - e[i].count + r / s.group, low = s.window ? std::max(0, p - s.window + 1) : 0;
+          if (p < 0) continue;
+          CHECK(span.lo * s.slots <= low && p < span.hi * s.slots && p < span.seen && span.seen <= e[i].length);
+        }
+      }
+    CHECK(tasks == got.size());
+  }
+}
+"""
+
+
+def test_every_block_of_every_task_has_one_workgroup(tmp_path):
+    """csrc/paged_plan.h on random batches: the runs cover every task's blocks once and in order, no two parts share a
+    place in the workspace, the tasks' tickets are their own and count the parts that arrive."""
+    (tmp_path / "plan.cpp").write_text(PLAN)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT / 'hawkpoint-npu-llm_amd' / 'csrc'}",
+                    str(tmp_path / "plan.cpp"), "-o", str(tmp_path / "plan")], check=True)
+    done = subprocess.run([str(tmp_path / "plan")], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout
