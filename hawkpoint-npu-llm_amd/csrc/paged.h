@@ -38,6 +38,7 @@ struct PagedAttnArgs {
   float* lse;
   int64_t q_stride, out_stride;
   int q_heads, group, window, max_new;
+  int rows_min, rows_max;  // set by the launch: rows (tokens x group) of the entries it takes
   float scale;
   void* workspace;
 };

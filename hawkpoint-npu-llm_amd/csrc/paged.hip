@@ -602,6 +602,10 @@ int hk_paged_attention(const hk_paged_cache* cache, int32_t layer, const uint16_
   HK_TRY(check_rows(who, "out", out, out_stride, width));
   HK_TRY(check_workspace(who, workspace));
   if (max_new < 1) return fail("hk_paged_attention: max_new must be positive");
+  if ((int64_t)tokens * q_heads > INT32_MAX) {
+    set_error("hk_paged_attention: more than 2^31 - 1 rows (tokens x q_heads)");
+    return HK_ERR_UNSUPPORTED;
+  }
   if (window < 0) return fail("hk_paged_attention: negative window");
   if (!std::isfinite(scale) || !(scale > 0.0f)) return fail("hk_paged_attention: scale must be finite and positive");
   if (n == 0 || tokens == 0) return 0;

@@ -54,6 +54,12 @@ __device__ __forceinline__ Entry load_entry(const PagedAttnArgs& a, int b) {
   return {uniform(s.x), uniform(r.x), {uniform(s.y), uniform(r.y - r.x)}};
 }
 
+// Whether an entry of `count` rows is this launch's (a batch of long and short
+// entries is two launches).
+__device__ __forceinline__ bool takes(const PagedAttnArgs& a, int count) {
+  return count > 0 && count * a.group >= a.rows_min && count * a.group <= a.rows_max;
+}
+
 // Sum of v over the workgroup in every thread, and the sum of the threads
 // before this one.
 __device__ __forceinline__ int64_t scan(int64_t v, int64_t* sums, int64_t& total) {
@@ -93,7 +99,7 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
   auto units = [&](int b) -> int64_t {
     if (b >= n) return 0;
     const int2 r = entry_rows(a.b, b);
-    if (r.y == r.x) return 0;
+    if (!takes(a, r.y - r.x)) return 0;
     return s.heads * plan_head_units(s, {entry_seq(a.c, a.b, b).y, r.y - r.x});
   };
   // (up to as many entries as threads, the units are worked out once)
@@ -145,7 +151,7 @@ __device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShap
   p.head = 0;
   while (++p.entry < a.b.n) {
     run.entry = load_entry(a, p.entry);
-    if (run.entry.e.count > 0) return;
+    if (takes(a, run.entry.e.count)) return;
   }
 }
 
@@ -200,11 +206,12 @@ struct Narrow {
   static constexpr int kPart = kRows * (D + 2);
 };
 
-// The position of 16-byte chunk c of V row r in LDS: c ^ key, so that the four
-// rows of a transposed read lie in different banks.
+// The position of 16-byte chunk c of V row r in LDS: c ^ key (an even number),
+// so that the rows of a transposed read, 32 bytes of each of eight, lie in
+// different banks, four by four and all eight.
 template <int D>
 __device__ __forceinline__ int v_key(int r) {
-  return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+  return D == 128 ? 2 * (r & 7) : 2 * (((r >> 1) & 3) ^ (2 * (r & 1)));
 }
 
 template <int D, bool E4M3, int NQ>
@@ -540,24 +547,416 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
   }
 }
 
-// Partial results and tickets of the largest launch fit the workspace.
-constexpr int kNarrowGroups[3] = {768, 512, 256};  // NQ 1, 2, 4: what the GPU holds at once
-template <int NQ, int GROUPS>
-constexpr bool fits() {
-  return GROUPS <= kPagedTicketWords && GROUPS % 8 == 0 &&
-         4ll * kPagedTicketWords + 2ll * GROUPS * Narrow<128, false, NQ>::kPart * 4 <= HK_PAGED_WORKSPACE;
-}
-static_assert(fits<1, kNarrowGroups[0]>() && fits<2, kNarrowGroups[1]>() && fits<4, kNarrowGroups[2]>(), "workspace");
+// ---- more rows: the waves share the rows ----
+//
+// A workgroup takes a tile of 128 QB rows, a wave 32 QB of them (QB columns of
+// v_mfma_f32_32x32x16_bf16), and goes through the slots 64 at a time.  K and V
+// come through registers into two LDS buffers, a block ahead, one barrier per
+// block; a fragment of either serves QB products.  LDS reads bound the loop at
+// QB 1 (a fragment of 1 KiB per product of 32 cycles and wave is all that a CU
+// reads), so ...
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int kWideSlots = 64;
 
+template <int D, int QB>
+struct Wide {
+  static constexpr int kRows = 128 * QB;
+  static constexpr int kBuf = kWideSlots * D;  // bf16 of one of K, V
+  // floats of a part: O, max and sum per lane
+  static constexpr int kLaneFloats = QB * (D / 2 + 2);
+  static constexpr int kPart = kThreads * kLaneFloats;
+};
+
+// Positions of the 16-byte chunks of K and V rows: a K fragment read is one
+// chunk of 32 rows, a transposed V read 32 bytes of each of four rows twice.
+template <int D>
+__device__ __forceinline__ int wide_k_key(int r) {
+  return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1);
+}
+template <int D>
+__device__ __forceinline__ int wide_v_key(int r) {
+  return D == 128 ? 2 * (2 * (r & 1) + 5 * ((r >> 1) & 1)) : 2 * (r & 3);
+}
+
+__device__ __forceinline__ float half_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+template <int D, bool E4M3, int QB>
+__global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(PagedAttnArgs a) {
+  using W = Wide<D, QB>;
+  constexpr int kRowBytes = D * (E4M3 ? 1 : 2), kLoads = kRowBytes / 64, kSteps = D / 16, kDims = D / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
+  __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
+  __shared__ int bad_lds[2][kWaves];
+  __shared__ int last;
+  const PlanShape shape = {a.c.kv_heads, a.group, a.window, W::kRows, kWideSlots};
+  const int w = run_of_group();
+  Run run;
+  if (!plan_run(a, shape, w, gridDim.x, 4, run)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
+  const int shift = a.c.page_shift, mask = (1 << shift) - 1;
+  float* const parts = static_cast<float*>(a.workspace) + kPagedTicketWords;
+  unsigned* const tickets = static_cast<unsigned*>(a.workspace);
+
+  while (run.unit < run.end) {
+    const PlanSpan span = plan_span(shape, run.entry.e, run.place.tile);
+    const int units = plan_units(span);
+    const int take = (int)min((int64_t)(units - run.place.at), run.end - run.unit);
+    const int g = run.place.head, r0 = run.place.tile * W::kRows;
+    const int rows = min(W::kRows, run.entry.e.count * a.group - r0);
+    const int pos0 = run.entry.e.length - run.entry.e.count;
+    const int kb0 = span.lo + run.place.at, kb1 = span.hi > span.lo ? kb0 + take : kb0;
+    const int32_t* const table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
+    const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
+    // the wave's rows [w0, w1) of the tile, and the positions they span
+    const int w0 = wave * 32 * QB, w1 = min(rows, w0 + 32 * QB);
+    const int wave_lo = pos0 + (r0 + w0) / a.group, wave_hi = w1 > w0 ? pos0 + (r0 + w1 - 1) / a.group : -1;
+    const int tile_lo = pos0 + r0 / a.group, tile_hi = pos0 + (r0 + rows - 1) / a.group;
+
+    int pos[QB], low[QB];
+    bf16x8 qf[QB][kSteps];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const int at = w0 + 32 * b + col, r = r0 + at, tok = r / a.group;
+      const bool ok = at < rows;
+      pos[b] = ok ? pos0 + tok : -1;
+      low[b] = a.window > 0 ? pos[b] - a.window : -1;
+      const uint16_t* q = a.q + (run.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) qf[b][s] = __builtin_bit_cast(bf16x8, load16(q + 16 * s + 8 * half));
+    }
+    float m_run[QB], l_run[QB];
+    f32x16 o[QB][kDims];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      m_run[b] = -INFINITY;
+      l_run[b] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
+    }
+
+    // wave w loads slots 16 w .. of a block (one page's): resources that end
+    // with the rows below span.seen, so later slots and absent pages read zero
+    u32x4 kr[kLoads], vr[kLoads];
+    auto load_block = [&](int s0) {
+      const int s = s0 + 16 * wave;
+      const int page = s < span.seen ? uniform(table[s >> shift]) : -1;
+      const bool on = (unsigned)page < (unsigned)a.c.pages;
+      const int bytes = on ? min(16, span.seen - s) * kRowBytes : 0;
+      const int64_t at = on ? page * a.c.page_bytes + (((int64_t)g << shift) + (s & mask)) * kRowBytes : 0;
+      const __amdgpu_buffer_rsrc_t kres = rsrc(a.c.k + at, bytes), vres = rsrc(a.c.v + at, bytes);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kres, 16 * lane + 1024 * i, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, 0);
+    };
+    // a block that every row of the tile sees whole (its pages apart)
+    auto all_see = [&](int s0, int lo, int hi) {
+      return s0 + kWideSlots - 1 <= lo && (a.window == 0 || s0 > hi - a.window);
+    };
+    auto store_block = [&](int s0, int buf) {
+      bool bad = false;
+      const bool whole = all_see(s0, tile_lo, tile_hi);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int b = 16 * lane + 1024 * i, r = 16 * wave + b / kRowBytes, c = b % kRowBytes / 16;
+        uint16_t *krow = &ks_lds[buf][r * D], *vrow = &vs_lds[buf][r * D];
+        if constexpr (E4M3) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const u32x2_t k0 = e4m3_bf16(kr[i][2 * e]), k1 = e4m3_bf16(kr[i][2 * e + 1]);
+            *reinterpret_cast<u32x4*>(krow + 8 * ((2 * c + e) ^ wide_k_key<D>(r))) = u32x4{k0.x, k0.y, k1.x, k1.y};
+            const u32x2_t v0 = e4m3_bf16(vr[i][2 * e]), v1 = e4m3_bf16(vr[i][2 * e + 1]);
+            const u32x4 v = {v0.x, v0.y, v1.x, v1.y};
+            *reinterpret_cast<u32x4*>(vrow + 8 * ((2 * c + e) ^ wide_v_key<D>(r))) = v;
+            if (!whole) bad |= not_finite(v);
+          }
+        } else {
+          *reinterpret_cast<u32x4*>(krow + 8 * (c ^ wide_k_key<D>(r))) = kr[i];
+          *reinterpret_cast<u32x4*>(vrow + 8 * (c ^ wide_v_key<D>(r))) = vr[i];
+          if (!whole) bad |= not_finite(vr[i]);
+        }
+      }
+      if (!whole) {
+        const int any = __any(bad);
+        if (lane == 0) bad_lds[buf][wave] = any;
+      }
+    };
+
+    if (kb0 < kb1) {
+      load_block(kb0 * kWideSlots);
+      store_block(kb0 * kWideSlots, 0);
+    }
+    for (int kb = kb0, buf = 0; kb < kb1; ++kb, buf ^= 1) {
+      const int s0 = kb * kWideSlots;
+      __syncthreads();  // the block is there, and the other buffer has been read
+      if (kb + 1 < kb1) load_block(s0 + kWideSlots);
+      if (s0 <= wave_hi) {
+        // bit h: slots 16 h .. of the block have a page
+        int there = 0;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int s = s0 + 16 * h;
+          if (s < span.seen && (unsigned)uniform(table[s >> shift]) < (unsigned)a.c.pages) there |= 1 << h;
+        }
+        // S^T: lane holds slots 32 t + 8 (i / 4) + 4 half + i % 4 of row col
+        f32x16 sv[QB][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sv[b][t][i] = 0.0f;
+          const int r = 32 * t + col;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&ks_lds[buf][r * D + 8 * ((2 * s + half) ^ wide_k_key<D>(r))]);
+#pragma unroll
+            for (int b = 0; b < QB; ++b) sv[b][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[b][s], sv[b][t], 0, 0, 0);
+          }
+        }
+        const bool whole = all_see(s0, wave_lo, wave_hi) && there == 15;
+        auto sees = [&](int b, int s) {
+          return (s <= pos[b]) & (s > low[b]) & (bool)((there >> ((s >> 4) & 3)) & 1);
+        };
+        if (!whole) {
+#pragma unroll
+          for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                sv[b][t][i] = sees(b, s0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) ? sv[b][t][i] : -INFINITY;
+        }
+        bf16x8 pf[QB][4];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sv[b][t][i]);
+          const float m_new = fmaxf(m_run[b], half_max(mx) * ks), m_use = finite_max(m_new);
+          const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_use);
+          float rs = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              sv[b][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[b][t][i], ks, -m_use));
+              rs += sv[b][t][i];
+            }
+          l_run[b] = l_run[b] * alpha + rs;
+          m_run[b] = m_new;
+          if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) o[b][d] *= alpha;
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            u32x4 pw;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              pw[e] = f32x2_to_bf16x2(sv[b][t >> 1][8 * (t & 1) + 2 * e], sv[b][t >> 1][8 * (t & 1) + 2 * e + 1]);
+            pf[b][t] = __builtin_bit_cast(bf16x8, pw);
+          }
+        }
+        bool slow = false;
+        if (!whole && !all_see(s0, tile_lo, tile_hi)) {
+#pragma unroll
+          for (int v = 0; v < kWaves; ++v) slow |= bad_lds[buf][v] != 0;
+        }
+        if (!uniform((int)slow)) {
+          // k index 8 half + e of product t stands for slot 16 t + 8 (e / 4) +
+          // 4 half + e % 4, the probabilities this lane holds; a group of 16
+          // lanes reads 4 slots of 16 dimensions, transposed
+          const int ra = 4 * half + ((lane & 15) >> 2), dd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+              const int r1 = 16 * t + ra, r2 = r1 + 8, dim = 32 * d + dd;
+              const v4s16 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r1 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r1)) + (dim & 7)]);
+              const v4s16 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r2 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r2)) + (dim & 7)]);
+              const u32x2_t w0 = __builtin_bit_cast(u32x2_t, t0), w1 = __builtin_bit_cast(u32x2_t, t1);
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{w0.x, w0.y, w1.x, w1.y});
+#pragma unroll
+              for (int b = 0; b < QB; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[b][t], o[b][d], 0, 0, 0);
+            }
+        } else {
+          // an infinity or NaN in a block that not every row sees whole: slot by
+          // slot, so that it reaches the rows that see it and no other
+#pragma unroll
+          for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              for (int j = 0; j < 16; ++j) {
+                const u32x4 pw = __builtin_bit_cast(u32x4, pf[b][t]);
+                const int e = 4 * (j >> 3) + (j & 3), s = 16 * t + j;
+                const uint32_t word = e < 2 ? pw[0] : e < 4 ? pw[1] : e < 6 ? pw[2] : pw[3];
+                const float mine = (e & 1) ? bf_hi(word) : bf_lo(word);
+                const float pj = __shfl(mine, col + 32 * ((j >> 2) & 1), 64);
+                const bool on = sees(b, s0 + s);
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const int dim = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+                    const float v = bf16_to_f32(vs_lds[buf][s * D + 8 * ((dim >> 3) ^ wide_v_key<D>(s)) + (dim & 7)]);
+                    const float y = fmaf(pj, v, o[b][d][i]);
+                    o[b][d][i] = on ? y : o[b][d][i];
+                  }
+              }
+        }
+      }
+      if (kb + 1 < kb1) store_block(s0 + kWideSlots, buf ^ 1);
+    }
+
+    const bool cut = take < units;
+    const PlanParts pp = plan_parts(run.place.start, units, run.per);
+#pragma unroll
+    for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
+    bool write = !cut;
+    if (cut) {
+      // the parts meet lane by lane: word i of lane t at (i * threads + t) * 4
+      // floats
+      const auto part = [&](int v) {
+        return rsrc(parts + (int64_t)plan_slot(run.place.start, v, run.per) * W::kPart, W::kPart * 4);
+      };
+      const __amdgpu_buffer_rsrc_t mine = part(w);
+      constexpr int kQuads = D / 8;  // 16-byte words of O per lane and QB
+      if (wave_hi >= 0) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+#pragma unroll
+          for (int i = 0; i < kQuads; ++i) {
+            const f32x16& x = o[b][i / 4];
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u32x4{__float_as_uint(x[4 * (i % 4)]), __float_as_uint(x[4 * (i % 4) + 1]), __float_as_uint(x[4 * (i % 4) + 2]),
+                      __float_as_uint(x[4 * (i % 4) + 3])},
+                mine, 16 * tid, 16 * kThreads * (b * kQuads + i), kSc1);
+          }
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(m_run[b]), __float_as_uint(l_run[b])}, mine,
+                                                16 * kThreads * QB * kQuads + 8 * tid, 8 * kThreads * b, kSc1);
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // every wave's stores have completed
+      if (tid == 0)
+        last = __hip_atomic_fetch_add(tickets + pp.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+               (unsigned)(pp.count - 1);
+      __syncthreads();
+      write = last != 0;
+      if (write) {
+        if (wave_hi >= 0) {
+#pragma unroll
+          for (int b = 0; b < QB; ++b) {
+            const int ml = 16 * kThreads * QB * kQuads + 8 * tid;
+            float m = -INFINITY;
+            for (int k = 0; k < pp.count; ++k)
+              m = fmaxf(m, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part(pp.first + k), ml, 8 * kThreads * b, kSc1)));
+            float l = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
+            for (int k = 0; k < pp.count; ++k) {
+              const __amdgpu_buffer_rsrc_t res = part(pp.first + k);
+              const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(res, ml, 8 * kThreads * b, kSc1);
+              const float f = __builtin_amdgcn_exp2f(__uint_as_float(x.x) - finite_max(m));
+              l = fmaf(__uint_as_float(x.y), f, l);
+#pragma unroll
+              for (int i = 0; i < kQuads; ++i) {
+                const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(res, 16 * tid, 16 * kThreads * (b * kQuads + i), kSc1);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  o[b][i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[c]), f, o[b][i / 4][4 * (i % 4) + c]);
+              }
+            }
+            m_run[b] = m;
+            l_run[b] = l;
+          }
+        }
+        if (tid == 0) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    if (write) {
+      const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        const int at = w0 + 32 * b + col;
+        if (at >= rows) continue;
+        const int tok = (r0 + at) / a.group, h = g * a.group + (r0 + at) - tok * a.group;
+        const int64_t row = run.entry.row0 + tok;
+        const float l = l_run[b], f = l == 0.0f ? 0.0f : vs / l;
+        uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x16& x = o[b][d];
+            u32x2_t y = {f32x2_to_bf16x2(x[4 * i] * f, x[4 * i + 1] * f), f32x2_to_bf16x2(x[4 * i + 2] * f, x[4 * i + 3] * f)};
+            if (l == 0.0f) y = u32x2_t{0u, 0u};
+            stg(reinterpret_cast<u32x2_t*>(dst + 32 * d + 8 * i), y);
+          }
+        if (a.lse && half == 0)
+          stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m_run[b] + __builtin_amdgcn_logf(l)) * kLn2);
+      }
+    }
+    __syncthreads();  // the buffers have been read
+    run.unit += take;
+    if (run.unit < run.end) plan_next(a, shape, run, units);
+  }
+}
+
+// Launches: narrow forms by rows, as many workgroups as the GPU holds at once.
+constexpr int kNarrowGroups[3] = {768, 512, 256};  // NQ 1, 2, 4
+constexpr int kWideQB = 1, kWideGroups = 512;
+constexpr bool fits(long long groups, long long part) {
+  return groups <= kPagedTicketWords && groups % 8 == 0 &&
+         4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
+}
+static_assert(fits(kNarrowGroups[0], Narrow<128, false, 1>::kPart) && fits(kNarrowGroups[1], Narrow<128, false, 2>::kPart) &&
+                  fits(kNarrowGroups[2], Narrow<128, false, 4>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
+              "partial results and tickets fit the workspace");
+
+// One launch for the entries of rows_min .. rows_max rows, `rows` of them at
+// most as far as the caller knows.
 template <int D, bool E4M3>
-void launch(const PagedAttnArgs& a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.max_new * a.group;
+void narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
   if (rows <= 16)
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kNarrowGroups[0]), dim3(kThreads), 0, stream, a);
   else if (rows <= 32)
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kNarrowGroups[1]), dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 4>), dim3(kNarrowGroups[2]), dim3(kThreads), 0, stream, a);
+}
+
+template <int D, bool E4M3>
+void launch(PagedAttnArgs a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.max_new * a.group;
+  a.rows_min = 1;
+  a.rows_max = INT32_MAX;
+  if (rows <= 64) return narrow<D, E4M3>(a, rows, stream);
+  // entries of a few rows beside longer ones: a launch of their own
+  const int few = a.group <= 16 ? 16 : a.group <= 32 ? 32 : 64;
+  if (a.b.n > 1 && a.group <= few) {
+    PagedAttnArgs b = a;
+    b.rows_max = few;
+    a.rows_min = few + 1;
+    narrow<D, E4M3>(b, few, stream);
+  }
+  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3, kWideQB>), dim3(kWideGroups), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
