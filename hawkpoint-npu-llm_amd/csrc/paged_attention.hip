@@ -182,6 +182,55 @@ __device__ __forceinline__ u32x2_t e4m3_bf16(uint32_t w) {
                  __builtin_amdgcn_perm(__float_as_uint(hi.y), __float_as_uint(hi.x), kTops)};
 }
 
+// The rows [r0, r0 + rows) of kv head g once more, a wave per row, 64 slots at a
+// time: a lane per slot for the scores, D / 64 dimensions per lane for P @ V.
+// For tasks whose tiles hold an infinity or NaN that only some of their rows
+// see: in a matrix product it would reach the others as 0 * inf.
+template <int D, bool E4M3>
+__device__ __forceinline__ float pool_value(const char* p, int i) {
+  if constexpr (E4M3) return __builtin_amdgcn_cvt_f32_fp8(ldg(reinterpret_cast<const uint8_t*>(p) + i), 0);
+  return bf16_to_f32(ldg(reinterpret_cast<const uint16_t*>(p) + i));
+}
+template <int D, bool E4M3>
+__device__ __forceinline__ void rows_again(const PagedAttnArgs& a, const Entry& en, int g, int r0, int rows) {
+  constexpr int kPer = D / 64;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), shift = a.c.page_shift;
+  const int32_t* const table = a.c.table + (int64_t)max(en.seq, 0) * a.c.width;
+  const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e, vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+  for (int r = r0 + wave; r < r0 + rows; r += kWaves) {
+    const int tok = r / a.group, h = g * a.group + r - tok * a.group, p = en.e.length - en.e.count + tok;
+    const int64_t row = en.row0 + tok;
+    const uint16_t* q = a.q + row * a.q_stride + h * D;
+    float m = -INFINITY, l = 0.0f, o[kPer] = {};
+    for (int j0 = a.window > 0 ? max(0, p - a.window + 1) : 0; j0 <= p; j0 += 64) {
+      const int j = j0 + lane, page = j <= p ? table[j >> shift] : -1;
+      const bool on = (unsigned)page < (unsigned)a.c.pages;
+      const int64_t off = on ? page * a.c.page_bytes + (((int64_t)g << shift) + (j & ((1 << shift) - 1))) * D * a.c.elt : 0;
+      float d = 0.0f;
+      if (on)
+        for (int i = 0; i < D; ++i) d = fmaf(bf16_to_f32(q[i]), pool_value<D, E4M3>(a.c.k + off, i), d);
+      const float sc = on ? d * ks : -INFINITY;
+      const float m_new = fmaxf(m, group_max<64>(sc)), f = __builtin_amdgcn_exp2f(m - finite_max(m_new));
+      const float e = on ? __builtin_amdgcn_exp2f(sc - finite_max(m_new)) : 0.0f;
+      l = l * f + group_sum<64>(e);
+      m = m_new;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) o[k] *= f;
+      for (int i = 0; i < 64; ++i) {
+        if (!__shfl((int)on, i, 64)) continue;
+        const float x = __shfl(e, i, 64);
+        const int64_t at = (int64_t)((uint64_t)(uint32_t)__shfl((int)(off >> 32), i, 64) << 32 | (uint32_t)__shfl((int)off, i, 64));
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) o[k] = fmaf(x, pool_value<D, E4M3>(a.c.v + at, lane + 64 * k), o[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      a.out[row * a.out_stride + h * D + lane + 64 * k] = (uint16_t)f32_to_bf16(l == 0.0f ? 0.0f : o[k] / l * vs);
+    if (a.lse && lane == 0) a.lse[row * a.q_heads + h] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+}
+
 // ---- up to 64 rows: the waves share the slots ----
 //
 // A wave takes 32 slots at a time: K straight into the MFMA's left operand
@@ -219,7 +268,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
   using N = Narrow<D, E4M3, NQ>;
   __shared__ __attribute__((aligned(16))) char lds[kWaves][N::kLds];
   __shared__ float wm[kWaves][N::kRows], wl[kWaves][N::kRows];
-  __shared__ int last;
+  __shared__ int last, again[kWaves], redo;
   const PlanShape shape = {a.c.kv_heads, a.group, a.window, N::kRows, kWaves * kNarrowSlots};
   const int w = run_of_group();
   Run run;
@@ -293,6 +342,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
       }
     };
 
+    bool poison = false;
     const int s_end = min(kb1 * kWaves * kNarrowSlots, span.seen);
     int s0 = (kb0 * kWaves + wave) * kNarrowSlots;
     if (s0 < s_end) load_tile(s0);
@@ -319,8 +369,8 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
         }
       }
       // V into LDS (the reads of the tile before are done: their values have
-      // been used).  Slots that not every row sees are the only ones whose
-      // values may not reach a product with 0.
+      // been used).  Where not every row sees every slot, an infinity or NaN
+      // among the values is noted for rows_again.
       const int tok0 = r0 / a.group, tok1 = (r0 + rows - 1) / a.group;
       const bool whole = s0 + kNarrowSlots - 1 <= pos0 + tok0 && there == 3 &&
                          (a.window == 0 || s0 > pos0 + tok1 - a.window);
@@ -349,7 +399,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
       auto sees = [&](int n, int s) {
         return (s <= pos[n]) & (s > low[n]) & (bool)((there >> ((s >> 4) & 1)) & 1);
       };
-      const bool slow = !whole && __any(bad);
+      poison |= bad;
       bf16x8 pf[NQ];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -378,7 +428,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
         pf[n] = __builtin_bit_cast(bf16x8, u32x4{f32x2_to_bf16x2(p[0], p[1]), f32x2_to_bf16x2(p[2], p[3]),
                                                  f32x2_to_bf16x2(p[4], p[5]), f32x2_to_bf16x2(p[6], p[7])});
       }
-      if (!slow) {
+      {
         // k index 8 quad + e of the product stands for slot 16 (e / 4) + 4 quad
         // + e % 4, the probabilities this lane holds; lane col of a group of 16
         // reads 4 slots of dimension 16 d + col
@@ -396,27 +446,6 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
 #pragma unroll
           for (int n = 0; n < NQ; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[n][d], 0, 0, 0);
         }
-      } else {
-        // an infinity or NaN in a tile that not every row sees whole: slot by
-        // slot, so that it reaches the rows that see it and no other
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-          for (int j = 0; j < kNarrowSlots; ++j) {
-            const u32x4 pw = __builtin_bit_cast(u32x4, pf[n]);
-            const int e = 4 * (j >> 4) + (j & 3);
-            const uint32_t word = e < 2 ? pw[0] : e < 4 ? pw[1] : e < 6 ? pw[2] : pw[3];
-            const float mine = (e & 1) ? bf_hi(word) : bf_lo(word);
-            const float pj = __shfl(mine, col + 16 * ((j >> 2) & 3), 64);
-            if (sees(n, s0 + j)) {
-#pragma unroll
-              for (int d = 0; d < N::kDims; ++d) {
-                const int dim = 16 * d + 4 * quad;
-                const uint16_t* v = reinterpret_cast<const uint16_t*>(mylds + j * D * 2 + 16 * ((dim >> 3) ^ v_key<D>(j))) + (dim & 7);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[n][d][r] = fmaf(pj, bf16_to_f32(v[r]), o[n][d][r]);
-              }
-            }
-          }
       }
     }
 
@@ -428,6 +457,10 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
         wm[wave][16 * n + col] = m_run[n];
         wl[wave][16 * n + col] = l;
       }
+    }
+    {
+      const int any = __any(poison);
+      if (lane == 0) again[wave] = any;
     }
     const bool cut = take < units;
     const PlanParts pp = plan_parts(run.place.start, units, run.per);
@@ -478,8 +511,10 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
           for (int k = 0; k < 4; ++k) x[i + k] = fmaf(y[k], f, x[i + k]);
         }
       }
+      const bool note = again[0] | again[1] | again[2] | again[3];
       if (!cut) {
-        finish(r, x, m, l);
+        if (!note) finish(r, x, m, l);
+        if (tid == 0) redo = note;
         continue;
       }
 #pragma unroll
@@ -488,7 +523,8 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
             u32x4{__float_as_uint(x[i]), __float_as_uint(x[i + 1]), __float_as_uint(x[i + 2]), __float_as_uint(x[i + 3])},
             mres, 4 * (r * D + od + i), 0, kSc1);
       if ((tid & 15) == 0) {
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m), mres, 4 * (N::kRows * D + r), 0, kSc1);
+        // (a NaN in the place of a maximum, which none is, passes the note on)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(note ? NAN : m), mres, 4 * (N::kRows * D + r), 0, kSc1);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), mres, 4 * (N::kRows * (D + 1) + r), 0, kSc1);
       }
     }
@@ -500,6 +536,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
                (unsigned)(pp.count - 1);
       __syncthreads();
       if (last) {
+        bool note = false;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           const int r = 16 * n + orow;
@@ -522,7 +559,10 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
             }
             float m_new = m;
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) m_new = fmaxf(m_new, pm[k]);
+            for (int k = 0; k < kBatch; ++k) {
+              m_new = fmaxf(m_new, pm[k]);
+              note |= pm[k] != pm[k];
+            }
             const float f0 = __builtin_amdgcn_exp2f(m - finite_max(m_new));
             l *= f0;
 #pragma unroll
@@ -537,11 +577,16 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
               for (int i = 0; i < kPer; ++i) x[i] = fmaf(__uint_as_float(px[k][i / 4][i % 4]), f, x[i]);
             }
           }
-          finish(r, x, m, l);
+          if (!note) finish(r, x, m, l);
         }
-        if (tid == 0) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) {  // (its row is there, and a note is in every row)
+          redo = note;
+          __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
       }
     }
+    if ((!cut || last) && redo) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
     run.unit += take;
     if (run.unit < run.end) plan_next(a, shape, run, units);
   }
@@ -594,7 +639,7 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
   __shared__ int bad_lds[2][kWaves];
-  __shared__ int last;
+  __shared__ int last, again[kWaves];
   const PlanShape shape = {a.c.kv_heads, a.group, a.window, W::kRows, kWideSlots};
   const int w = run_of_group();
   Run run;
@@ -691,6 +736,7 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
       }
     };
 
+    int poison = 0;  // an infinity or NaN among values that not every row sees, for rows_again
     if (kb0 < kb1) {
       load_block(kb0 * kWideSlots);
       store_block(kb0 * kWideSlots, 0);
@@ -769,12 +815,11 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
             pf[b][t] = __builtin_bit_cast(bf16x8, pw);
           }
         }
-        bool slow = false;
         if (!whole && !all_see(s0, tile_lo, tile_hi)) {
 #pragma unroll
-          for (int v = 0; v < kWaves; ++v) slow |= bad_lds[buf][v] != 0;
+          for (int v = 0; v < kWaves; ++v) poison |= bad_lds[buf][v];
         }
-        if (!uniform((int)slow)) {
+        {
           // k index 8 half + e of product t stands for slot 16 t + 8 (e / 4) +
           // 4 half + e % 4, the probabilities this lane holds; a group of 16
           // lanes reads 4 slots of 16 dimensions, transposed
@@ -793,30 +838,6 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
 #pragma unroll
               for (int b = 0; b < QB; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[b][t], o[b][d], 0, 0, 0);
             }
-        } else {
-          // an infinity or NaN in a block that not every row sees whole: slot by
-          // slot, so that it reaches the rows that see it and no other
-#pragma unroll
-          for (int b = 0; b < QB; ++b)
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              for (int j = 0; j < 16; ++j) {
-                const u32x4 pw = __builtin_bit_cast(u32x4, pf[b][t]);
-                const int e = 4 * (j >> 3) + (j & 3), s = 16 * t + j;
-                const uint32_t word = e < 2 ? pw[0] : e < 4 ? pw[1] : e < 6 ? pw[2] : pw[3];
-                const float mine = (e & 1) ? bf_hi(word) : bf_lo(word);
-                const float pj = __shfl(mine, col + 32 * ((j >> 2) & 1), 64);
-                const bool on = sees(b, s0 + s);
-#pragma unroll
-                for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const int dim = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
-                    const float v = bf16_to_f32(vs_lds[buf][s * D + 8 * ((dim >> 3) ^ wide_v_key<D>(s)) + (dim & 7)]);
-                    const float y = fmaf(pj, v, o[b][d][i]);
-                    o[b][d][i] = on ? y : o[b][d][i];
-                  }
-              }
         }
       }
       if (kb + 1 < kb1) store_block(s0 + kWideSlots, buf ^ 1);
@@ -826,7 +847,9 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
     const PlanParts pp = plan_parts(run.place.start, units, run.per);
 #pragma unroll
     for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
-    bool write = !cut;
+    if (lane == 0) again[wave] = poison;
+    __syncthreads();  // the buffers have been read
+    bool note = again[0] | again[1] | again[2] | again[3], write = !cut;
     if (cut) {
       // the parts meet lane by lane: word i of lane t at (i * threads + t) * 4
       // floats
@@ -846,7 +869,8 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
                       __float_as_uint(x[4 * (i % 4) + 3])},
                 mine, 16 * tid, 16 * kThreads * (b * kQuads + i), kSc1);
           }
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(m_run[b]), __float_as_uint(l_run[b])}, mine,
+          // (a NaN in the place of a maximum, which none is, passes the note on)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(note ? NAN : m_run[b]), __float_as_uint(l_run[b])}, mine,
                                                 16 * kThreads * QB * kQuads + 8 * tid, 8 * kThreads * b, kSc1);
         }
       }
@@ -863,8 +887,11 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
           for (int b = 0; b < QB; ++b) {
             const int ml = 16 * kThreads * QB * kQuads + 8 * tid;
             float m = -INFINITY;
-            for (int k = 0; k < pp.count; ++k)
-              m = fmaxf(m, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part(pp.first + k), ml, 8 * kThreads * b, kSc1)));
+            for (int k = 0; k < pp.count; ++k) {
+              const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part(pp.first + k), ml, 8 * kThreads * b, kSc1));
+              m = fmaxf(m, x);
+              note |= x != x;
+            }
             float l = 0.0f;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
@@ -887,10 +914,17 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
             l_run[b] = l;
           }
         }
+        {
+          const int any = __any(note);
+          if (lane == 0) again[wave] = any;
+        }
+        __syncthreads();
+        note = again[0] | again[1] | again[2] | again[3];
         if (tid == 0) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
-    if (write) {
+    if (write && note) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
+    if (write && !note) {
       const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
 #pragma unroll
       for (int b = 0; b < QB; ++b) {
@@ -913,7 +947,7 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
           stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m_run[b] + __builtin_amdgcn_logf(l)) * kLn2);
       }
     }
-    __syncthreads();  // the buffers have been read
+    __syncthreads();  // (the notes have been read)
     run.unit += take;
     if (run.unit < run.end) plan_next(a, shape, run, units);
   }
