@@ -35,7 +35,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kSc1 = 16;  // buffer access cache policy: device scope
+// buffer access cache policies
+constexpr int kSc1 = 16;    // device scope
+constexpr int kStream = 2;  // read once: does not stay in the caches
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -94,13 +96,15 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
                                          Run& run) {
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found_start;
-  __shared__ int found;
+  __shared__ int found[5];
   const int n = a.b.n;
+  int2 rows, seq;
   auto units = [&](int b) -> int64_t {
     if (b >= n) return 0;
-    const int2 r = entry_rows(a.b, b);
-    if (!takes(a, r.y - r.x)) return 0;
-    return s.heads * plan_head_units(s, {entry_seq(a.c, a.b, b).y, r.y - r.x});
+    rows = entry_rows(a.b, b);
+    seq = entry_seq(a.c, a.b, b);
+    if (!takes(a, rows.y - rows.x)) return 0;
+    return s.heads * plan_head_units(s, {seq.y, rows.y - rows.x});
   };
   // (up to as many entries as threads, the units are worked out once)
   int64_t mine = units(threadIdx.x), total, before = scan(mine, sums, total);
@@ -124,18 +128,20 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
       mine = units(b0 + threadIdx.x);
       before = base + scan(mine, sums, chunk);
     } else if (n > kThreads) {
+      mine = units(threadIdx.x);
       scan(mine, sums, chunk);
     }
     if (before <= run.unit && run.unit < before + mine) {
-      found = b0 + threadIdx.x;
+      found[0] = b0 + threadIdx.x;
+      found[1] = seq.x, found[2] = rows.x, found[3] = seq.y, found[4] = rows.y - rows.x;
       found_start = before;
     }
     base += chunk;
   }
   __syncthreads();
-  const int b = uniform(found);
+  const int b = uniform(found[0]);
   const int64_t start = uniform(found_start);
-  run.entry = load_entry(a, b);
+  run.entry = {uniform(found[1]), uniform(found[2]), {uniform(found[3]), uniform(found[4])}};
   run.place = plan_find(s, run.entry.e, b, start, run.unit - start);
   return true;
 }
@@ -174,12 +180,47 @@ __device__ __forceinline__ bool not_finite(const u32x4& v) {
   return bad;
 }
 
-// Four e4m3 values as two bf16 pairs (exact: every e4m3 value is a bf16 value).
+// Four e4m3 values as two bf16 pairs (exact: every e4m3 value is a bf16 value;
+// v_cvt_scalef32_pk_bf16_fp8 with scale 1).
 __device__ __forceinline__ u32x2_t e4m3_bf16(uint32_t w) {
-  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-  constexpr uint32_t kTops = 0x07060302u;  // a float's high half is the exact bf16
-  return u32x2_t{__builtin_amdgcn_perm(__float_as_uint(lo.y), __float_as_uint(lo.x), kTops),
-                 __builtin_amdgcn_perm(__float_as_uint(hi.y), __float_as_uint(hi.x), kTops)};
+  return u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+}
+
+// ---- cut tasks ----
+
+// A task whose result is one of several parts: where it starts in the order of
+// units, and what is written when all parts are there.
+struct Pending {
+  int64_t start;
+  Entry entry;
+  int units, head, tile;
+};
+
+// Once the workgroup's parts are stored: draws the tickets of its (at most
+// two) cut tasks, and says which of them it has to join, as bits.  The stores
+// have completed before the tickets are drawn (device-coherent stores, no L2
+// write-back as a fence would do).  The joining workgroup leaves the ticket at
+// zero.
+__device__ __forceinline__ int draw_tickets(const PagedAttnArgs& a, const Pending (&pend)[2], int n, int64_t per, int* last) {
+  unsigned* const tickets = static_cast<unsigned*>(a.workspace);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if ((int)threadIdx.x < n) {
+    const Pending& p = threadIdx.x ? pend[1] : pend[0];
+    const PlanParts pp = plan_parts(p.start, p.units, per);
+    const bool is = __hip_atomic_fetch_add(tickets + pp.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                    (unsigned)(pp.count - 1);
+    if (is) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last[threadIdx.x] = is;
+  }
+  __syncthreads();
+  return (n > 0 && uniform(last[0]) ? 1 : 0) | (n > 1 && uniform(last[1]) ? 2 : 0);
+}
+
+// The partial results as one buffer; byte offset of workgroup w's part.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_of(const PagedAttnArgs& a) {
+  return rsrc(static_cast<char*>(a.workspace) + 4 * kPagedTicketWords, HK_PAGED_WORKSPACE - 4 * kPagedTicketWords);
 }
 
 // The rows [r0, r0 + rows) of kv head g once more, a wave per row, 64 slots at a
@@ -264,11 +305,13 @@ __device__ __forceinline__ int v_key(int r) {
 }
 
 template <int D, bool E4M3, int NQ>
-__global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs a) {
   using N = Narrow<D, E4M3, NQ>;
   __shared__ __attribute__((aligned(16))) char lds[kWaves][N::kLds];
   __shared__ float wm[kWaves][N::kRows], wl[kWaves][N::kRows];
-  __shared__ int last, again[kWaves], redo;
+  __shared__ int last[2], again[kWaves];
+  constexpr int kJoin = 32;  // parts at a time
+  static_assert(2 * 4 * kJoin * N::kRows <= kWaves * N::kLds, "the weights fit the waves' LDS rows");
   const PlanShape shape = {a.c.kv_heads, a.group, a.window, N::kRows, kWaves * kNarrowSlots};
   const int w = run_of_group();
   Run run;
@@ -276,8 +319,19 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, quad = lane >> 4;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
   char* const mylds = lds[wave];
-  float* const parts = static_cast<float*>(a.workspace) + kPagedTicketWords;
-  unsigned* const tickets = static_cast<unsigned*>(a.workspace);
+  const __amdgpu_buffer_rsrc_t parts = parts_of(a);
+  Pending pend[2];
+  int pending = 0;
+  // four dimensions of a finished row, and its lse
+  auto finish = [&](const Entry& en, int g, int r, int d, const f32x4& x, float m, float l) {
+    const int tok = r / a.group, h = g * a.group + r - tok * a.group;
+    const int64_t row = en.row0 + tok;
+    const float f = l == 0.0f ? 0.0f : (E4M3 ? a.c.v_scale[g] : 1.0f) / l;
+    u32x2_t y = {f32x2_to_bf16x2(x[0] * f, x[1] * f), f32x2_to_bf16x2(x[2] * f, x[3] * f)};
+    if (l == 0.0f) y = u32x2_t{0u, 0u};
+    stg(reinterpret_cast<u32x2_t*>(a.out + row * a.out_stride + h * D + d), y);
+    if (a.lse && d == 0) stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2);
+  };
 
   while (run.unit < run.end) {
     const PlanSpan span = plan_span(shape, run.entry.e, run.place.tile);
@@ -335,10 +389,10 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
         const __amdgpu_buffer_rsrc_t kres = rsrc(a.c.k + at, bytes), vres = rsrc(a.c.v + at, bytes);
 #pragma unroll
         for (int i = 0; i < N::kKLoads; ++i)
-          kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(kres, col * N::kRowBytes + 16 * quad + 64 * i, 0, 0);
+          kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(kres, col * N::kRowBytes + 16 * quad + 64 * i, 0, kStream);
 #pragma unroll
         for (int i = 0; i < N::kVLoads; ++i)
-          vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, 0);
+          vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, kStream);
       }
     };
 
@@ -463,29 +517,10 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
       if (lane == 0) again[wave] = any;
     }
     const bool cut = take < units;
-    const PlanParts pp = plan_parts(run.place.start, units, run.per);
-    const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+    const int slot = plan_slot(run.place.start, w, run.per) * (N::kPart * 4);
     constexpr int kPer = D / 16;  // outputs of a thread: dimensions kPer (tid % 16) .. of row tid / 16
     const int orow = tid >> 4, od = kPer * (tid & 15);
-    // a finished row: out and lse
-    auto finish = [&](int r, const float (&x)[kPer], float m, float l) {
-      const int tok = (r0 + r) / a.group, h = g * a.group + (r0 + r) % a.group;
-      const int64_t row = run.entry.row0 + tok;
-      const float f = l == 0.0f ? 0.0f : vs / l;
-      uint32_t ow[kPer / 2];
-#pragma unroll
-      for (int i = 0; i < kPer / 2; ++i)
-        ow[i] = l == 0.0f ? 0u : f32x2_to_bf16x2(x[2 * i] * f, x[2 * i + 1] * f);
-      uint16_t* dst = a.out + row * a.out_stride + h * D + od;
-      if constexpr (kPer == 8)
-        stg(reinterpret_cast<u32x4*>(dst), u32x4{ow[0], ow[1], ow[2], ow[3]});
-      else
-        stg(reinterpret_cast<u32x2_t*>(dst), u32x2_t{ow[0], ow[1]});
-      if (a.lse && (tid & 15) == 0)
-        stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2);
-    };
-    float* const mine = parts + (int64_t)plan_slot(run.place.start, w, run.per) * N::kPart;
-    const __amdgpu_buffer_rsrc_t mres = rsrc(mine, N::kPart * 4);
+    bool note = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       if (16 * n >= rows) break;
@@ -494,6 +529,7 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
 #pragma unroll
       for (int d = 0; d < N::kDims; ++d) *reinterpret_cast<f32x4*>(ow + 16 * d) = o[n][d];
       __syncthreads();
+      note = again[0] | again[1] | again[2] | again[3];
       const int r = 16 * n + orow;
       if (r >= rows) continue;
       float m = wm[0][r], l = 0.0f, x[kPer] = {};
@@ -511,84 +547,103 @@ __global__ __launch_bounds__(kThreads, NQ == 4 ? 1 : 2) void paged_narrow_kernel
           for (int k = 0; k < 4; ++k) x[i + k] = fmaf(y[k], f, x[i + k]);
         }
       }
-      const bool note = again[0] | again[1] | again[2] | again[3];
-      if (!cut) {
-        if (!note) finish(r, x, m, l);
-        if (tid == 0) redo = note;
-        continue;
-      }
 #pragma unroll
-      for (int i = 0; i < kPer; i += 4)
-        __builtin_amdgcn_raw_buffer_store_b128(
-            u32x4{__float_as_uint(x[i]), __float_as_uint(x[i + 1]), __float_as_uint(x[i + 2]), __float_as_uint(x[i + 3])},
-            mres, 4 * (r * D + od + i), 0, kSc1);
-      if ((tid & 15) == 0) {
+      for (int i = 0; i < kPer; i += 4) {
+        const f32x4 y = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+        if (cut)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, slot + 4 * (r * D + od + i), 0, kSc1);
+        else if (!note)
+          finish(run.entry, g, r0 + r, od + i, y, m, l);
+      }
+      if (cut && (tid & 15) == 0) {
         // (a NaN in the place of a maximum, which none is, passes the note on)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(note ? NAN : m), mres, 4 * (N::kRows * D + r), 0, kSc1);
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), mres, 4 * (N::kRows * (D + 1) + r), 0, kSc1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(note ? NAN : m), parts, slot + 4 * (N::kRows * D + r), 0, kSc1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), parts, slot + 4 * (N::kRows * (D + 1) + r), 0, kSc1);
       }
     }
-    if (cut) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (each wave's stores have completed)
     __syncthreads();  // the waves' V rows are free again
+    if (!cut && note) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
     if (cut) {
-      if (tid == 0)
-        last = __hip_atomic_fetch_add(tickets + pp.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-               (unsigned)(pp.count - 1);
-      __syncthreads();
-      if (last) {
-        bool note = false;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          const int r = 16 * n + orow;
-          if (r >= rows) break;
-          float m = -INFINITY, l = 0.0f, x[kPer] = {};
-          constexpr int kBatch = 4;
-          for (int k0 = 0; k0 < pp.count; k0 += kBatch) {
-            float pm[kBatch], pl[kBatch];
-            u32x4 px[kBatch][kPer / 4];
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int wk = pp.first + min(k0 + k, pp.count - 1);
-              const __amdgpu_buffer_rsrc_t res =
-                  rsrc(parts + (int64_t)plan_slot(run.place.start, wk, run.per) * N::kPart, N::kPart * 4);
-              pm[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(res, 4 * (N::kRows * D + r), 0, kSc1));
-              pl[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(res, 4 * (N::kRows * (D + 1) + r), 0, kSc1));
-#pragma unroll
-              for (int i = 0; i < kPer / 4; ++i)
-                px[k][i] = __builtin_amdgcn_raw_buffer_load_b128(res, 4 * (r * D + od + 4 * i), 0, kSc1);
-            }
-            float m_new = m;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              m_new = fmaxf(m_new, pm[k]);
-              note |= pm[k] != pm[k];
-            }
-            const float f0 = __builtin_amdgcn_exp2f(m - finite_max(m_new));
-            l *= f0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) x[i] *= f0;
-            m = m_new;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              if (k0 + k >= pp.count) break;
-              const float f = __builtin_amdgcn_exp2f(pm[k] - finite_max(m));
-              l = fmaf(pl[k], f, l);
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) x[i] = fmaf(__uint_as_float(px[k][i / 4][i % 4]), f, x[i]);
-            }
-          }
-          if (!note) finish(r, x, m, l);
-        }
-        if (tid == 0) {  // (its row is there, and a note is in every row)
-          redo = note;
-          __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-      }
+      const Pending p = {run.place.start, run.entry, units, g, run.place.tile};
+      if (pending == 0) pend[0] = p; else pend[1] = p;
+      ++pending;
     }
-    if ((!cut || last) && redo) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
     run.unit += take;
     if (run.unit < run.end) plan_next(a, shape, run, units);
+  }
+
+  const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
+  // joins a task's parts: their weights through LDS, 32 parts at a time, then
+  // four dimensions of a row per thread and step
+  float (&pm)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][0]);
+  float (&pl)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][sizeof(float) * kJoin * N::kRows]);
+  for (int j = 0; j < 2; ++j) {
+    if (!((join >> j) & 1)) continue;
+    const Pending& p = j ? pend[1] : pend[0];
+    const PlanParts pp = plan_parts(p.start, p.units, run.per);
+    const int r0 = p.tile * N::kRows, rows = min(N::kRows, p.entry.e.count * a.group - r0);
+    constexpr int kQuads = D / 4, kItems = N::kRows * kQuads / kThreads;
+    f32x4 x[kItems] = {};
+    int note = 0;
+    __syncthreads();  // (wm, wl and the weights of another task have been read)
+    if (tid < N::kRows) wm[0][tid] = -INFINITY, wl[0][tid] = 0.0f;
+    for (int k0 = 0; k0 < pp.count; k0 += kJoin) {
+      const int n = min(kJoin, pp.count - k0);
+      __syncthreads();
+      for (int i = tid; i < n * N::kRows; i += kThreads) {
+        const int k = i / N::kRows, r = i % N::kRows;
+        const int at = plan_slot(p.start, pp.first + k0 + k, run.per) * (N::kPart * 4);
+        pm[k][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * D + r), 0, kSc1));
+        pl[k][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * (D + 1) + r), 0, kSc1));
+      }
+      __syncthreads();
+      for (int k = 0; k < n; ++k) note |= pm[k][0] != pm[k][0];
+      __syncthreads();
+      if (tid < rows) {
+        const float m0 = wm[0][tid];
+        float m = m0;
+        for (int k = 0; k < n; ++k) m = fmaxf(m, pm[k][tid]);
+        const float f = __builtin_amdgcn_exp2f(m0 - finite_max(m));
+        float l = wl[0][tid] * f;
+        for (int k = 0; k < n; ++k) {
+          const float e = __builtin_amdgcn_exp2f(pm[k][tid] - finite_max(m));
+          l = fmaf(pl[k][tid], e, l);
+          pm[k][tid] = e;
+        }
+        wm[0][tid] = m, wl[0][tid] = l, wm[1][tid] = f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int r = (tid + i * kThreads) / kQuads, d = 4 * ((tid + i * kThreads) % kQuads);
+        if (r >= rows) break;
+        x[i] *= wm[1][r];
+        constexpr int kBatch = 8;
+        for (int q = 0; q < n; q += kBatch) {
+          u32x4 y[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+            y[k] = __builtin_amdgcn_raw_buffer_load_b128(
+                parts, plan_slot(p.start, pp.first + k0 + min(q + k, n - 1), run.per) * (N::kPart * 4) + 4 * (r * D + d), 0, kSc1);
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            if (q + k >= n) break;
+            const float f = pm[q + k][r];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[i][c] = fmaf(__uint_as_float(y[k][c]), f, x[i][c]);
+          }
+        }
+      }
+    }
+    if (note) {
+      rows_again<D, E4M3>(a, p.entry, p.head, r0, rows);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int r = (tid + i * kThreads) / kQuads, d = 4 * ((tid + i * kThreads) % kQuads);
+      if (r < rows) finish(p.entry, p.head, r0 + r, d, x[i], wm[0][r], wl[0][r]);
+    }
   }
 }
 
@@ -639,15 +694,41 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
   __shared__ int bad_lds[2][kWaves];
-  __shared__ int last, again[kWaves];
+  __shared__ int last[2], again[kWaves];
+  constexpr int kQuads = D / 8;  // 16-byte words of a part's O per lane and QB
   const PlanShape shape = {a.c.kv_heads, a.group, a.window, W::kRows, kWideSlots};
   const int w = run_of_group();
   Run run;
   if (!plan_run(a, shape, w, gridDim.x, 4, run)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
-  float* const parts = static_cast<float*>(a.workspace) + kPagedTicketWords;
-  unsigned* const tickets = static_cast<unsigned*>(a.workspace);
+  const __amdgpu_buffer_rsrc_t parts = parts_of(a);
+  Pending pend[2];
+  int pending = 0;
+  // the finished rows of a tile, and their lse
+  auto finish = [&](const Entry& en, int g, int r0, int rows, const f32x16 (&o)[QB][kDims], const float (&ms)[QB], const float (&ls)[QB]) {
+    const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const int at = 32 * (QB * wave + b) + col;
+      if (at >= rows) continue;
+      const int tok = (r0 + at) / a.group, h = g * a.group + (r0 + at) - tok * a.group;
+      const int64_t row = en.row0 + tok;
+      const float l = ls[b], f = l == 0.0f ? 0.0f : vs / l;
+      uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x16& x = o[b][d];
+          u32x2_t y = {f32x2_to_bf16x2(x[4 * i] * f, x[4 * i + 1] * f), f32x2_to_bf16x2(x[4 * i + 2] * f, x[4 * i + 3] * f)};
+          if (l == 0.0f) y = u32x2_t{0u, 0u};
+          stg(reinterpret_cast<u32x2_t*>(dst + 32 * d + 8 * i), y);
+        }
+      if (a.lse && half == 0)
+        stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (ms[b] + __builtin_amdgcn_logf(l)) * kLn2);
+    }
+  };
 
   while (run.unit < run.end) {
     const PlanSpan span = plan_span(shape, run.entry.e, run.place.tile);
@@ -844,124 +925,106 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
     }
 
     const bool cut = take < units;
-    const PlanParts pp = plan_parts(run.place.start, units, run.per);
 #pragma unroll
     for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
     if (lane == 0) again[wave] = poison;
     __syncthreads();  // the buffers have been read
-    bool note = again[0] | again[1] | again[2] | again[3], write = !cut;
+    const bool note = again[0] | again[1] | again[2] | again[3];
     if (cut) {
-      // the parts meet lane by lane: word i of lane t at (i * threads + t) * 4
-      // floats
-      const auto part = [&](int v) {
-        return rsrc(parts + (int64_t)plan_slot(run.place.start, v, run.per) * W::kPart, W::kPart * 4);
-      };
-      const __amdgpu_buffer_rsrc_t mine = part(w);
-      constexpr int kQuads = D / 8;  // 16-byte words of O per lane and QB
+      // parts lie lane by lane: word i of thread t at 16 (i threads + t) bytes
+      const int slot = plan_slot(run.place.start, w, run.per) * (W::kPart * 4);
       if (wave_hi >= 0) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
 #pragma unroll
           for (int i = 0; i < kQuads; ++i) {
             const f32x16& x = o[b][i / 4];
-            __builtin_amdgcn_raw_buffer_store_b128(
-                u32x4{__float_as_uint(x[4 * (i % 4)]), __float_as_uint(x[4 * (i % 4) + 1]), __float_as_uint(x[4 * (i % 4) + 2]),
-                      __float_as_uint(x[4 * (i % 4) + 3])},
-                mine, 16 * tid, 16 * kThreads * (b * kQuads + i), kSc1);
+            const f32x4 y = {x[4 * (i % 4)], x[4 * (i % 4) + 1], x[4 * (i % 4) + 2], x[4 * (i % 4) + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts,
+                                                   slot + 16 * (kThreads * (b * kQuads + i) + tid), 0, kSc1);
           }
           // (a NaN in the place of a maximum, which none is, passes the note on)
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(note ? NAN : m_run[b]), __float_as_uint(l_run[b])}, mine,
-                                                16 * kThreads * QB * kQuads + 8 * tid, 8 * kThreads * b, kSc1);
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(note ? NAN : m_run[b]), __float_as_uint(l_run[b])}, parts,
+                                                slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
         }
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // every wave's stores have completed
-      if (tid == 0)
-        last = __hip_atomic_fetch_add(tickets + pp.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-               (unsigned)(pp.count - 1);
-      __syncthreads();
-      write = last != 0;
-      if (write) {
-        if (wave_hi >= 0) {
-#pragma unroll
-          for (int b = 0; b < QB; ++b) {
-            const int ml = 16 * kThreads * QB * kQuads + 8 * tid;
-            float m = -INFINITY;
-            for (int k = 0; k < pp.count; ++k) {
-              const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part(pp.first + k), ml, 8 * kThreads * b, kSc1));
-              m = fmaxf(m, x);
-              note |= x != x;
-            }
-            float l = 0.0f;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
-            for (int k = 0; k < pp.count; ++k) {
-              const __amdgpu_buffer_rsrc_t res = part(pp.first + k);
-              const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(res, ml, 8 * kThreads * b, kSc1);
-              const float f = __builtin_amdgcn_exp2f(__uint_as_float(x.x) - finite_max(m));
-              l = fmaf(__uint_as_float(x.y), f, l);
-#pragma unroll
-              for (int i = 0; i < kQuads; ++i) {
-                const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(res, 16 * tid, 16 * kThreads * (b * kQuads + i), kSc1);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  o[b][i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[c]), f, o[b][i / 4][4 * (i % 4) + c]);
-              }
-            }
-            m_run[b] = m;
-            l_run[b] = l;
-          }
-        }
-        {
-          const int any = __any(note);
-          if (lane == 0) again[wave] = any;
-        }
-        __syncthreads();
-        note = again[0] | again[1] | again[2] | again[3];
-        if (tid == 0) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-    }
-    if (write && note) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
-    if (write && !note) {
-      const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
-#pragma unroll
-      for (int b = 0; b < QB; ++b) {
-        const int at = w0 + 32 * b + col;
-        if (at >= rows) continue;
-        const int tok = (r0 + at) / a.group, h = g * a.group + (r0 + at) - tok * a.group;
-        const int64_t row = run.entry.row0 + tok;
-        const float l = l_run[b], f = l == 0.0f ? 0.0f : vs / l;
-        uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x16& x = o[b][d];
-            u32x2_t y = {f32x2_to_bf16x2(x[4 * i] * f, x[4 * i + 1] * f), f32x2_to_bf16x2(x[4 * i + 2] * f, x[4 * i + 3] * f)};
-            if (l == 0.0f) y = u32x2_t{0u, 0u};
-            stg(reinterpret_cast<u32x2_t*>(dst + 32 * d + 8 * i), y);
-          }
-        if (a.lse && half == 0)
-          stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m_run[b] + __builtin_amdgcn_logf(l)) * kLn2);
-      }
+      const Pending p = {run.place.start, run.entry, units, g, run.place.tile};
+      if (pending == 0) pend[0] = p; else pend[1] = p;
+      ++pending;
+    } else if (note) {
+      rows_again<D, E4M3>(a, run.entry, g, r0, rows);
+    } else {
+      finish(run.entry, g, r0, rows, o, m_run, l_run);
     }
     __syncthreads();  // (the notes have been read)
     run.unit += take;
     if (run.unit < run.end) plan_next(a, shape, run, units);
   }
+
+  const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
+  for (int j = 0; j < 2; ++j) {
+    if (!((join >> j) & 1)) continue;
+    const Pending& p = j ? pend[1] : pend[0];
+    const PlanParts pp = plan_parts(p.start, p.units, run.per);
+    const int r0 = p.tile * W::kRows, rows = min(W::kRows, p.entry.e.count * a.group - r0);
+    // (a wave whose rows stand at negative positions has no part)
+    const bool has = p.entry.e.length - p.entry.e.count + (r0 + min(rows, 32 * QB * (wave + 1)) - 1) / a.group >= 0 &&
+                     rows > 32 * QB * wave;
+    float m[QB], l[QB];
+    f32x16 o[QB][kDims];
+    bool note = false;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      m[b] = -INFINITY;
+      l[b] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
+      if (!has) continue;
+      for (int k = 0; k < pp.count; ++k) {
+        const int slot = plan_slot(p.start, pp.first + k, run.per) * (W::kPart * 4);
+        const u32x2_t ml =
+            __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
+        u32x4 y[kQuads];
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+          y[i] = __builtin_amdgcn_raw_buffer_load_b128(parts, slot + 16 * (kThreads * (b * kQuads + i) + tid), 0, kSc1);
+        const float mk = __uint_as_float(ml.x), m_new = fmaxf(m[b], mk);
+        const float f0 = __builtin_amdgcn_exp2f(m[b] - finite_max(m_new)), f1 = __builtin_amdgcn_exp2f(mk - finite_max(m_new));
+        note |= mk != mk;
+        l[b] = l[b] * f0 + __uint_as_float(ml.y) * f1;
+        m[b] = m_new;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            o[b][i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[i][c]), f1, o[b][i / 4][4 * (i % 4) + c] * f0);
+      }
+    }
+    const int any = __any(note);
+    if (lane == 0) again[wave] = any;
+    __syncthreads();
+    if (again[0] | again[1] | again[2] | again[3])
+      rows_again<D, E4M3>(a, p.entry, p.head, r0, rows);
+    else
+      finish(p.entry, p.head, r0, rows, o, m, l);
+    __syncthreads();
+  }
 }
 
-// Launches: narrow forms by rows, as many workgroups as the GPU holds at once.
-constexpr int kNarrowGroups[3] = {768, 512, 256};  // NQ 1, 2, 4
+// Launches: as many workgroups as the GPU holds at once.
+template <int D, bool E4M3>
+constexpr int narrow_groups(int nq) {
+  return nq == 2 ? 512 : D == 64 ? 1024 : E4M3 ? 768 : 512;
+}
 constexpr int kWideQB = 1, kWideGroups = 512;
 constexpr bool fits(long long groups, long long part) {
   return groups <= kPagedTicketWords && groups % 8 == 0 &&
          4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
 }
-static_assert(fits(kNarrowGroups[0], Narrow<128, false, 1>::kPart) && fits(kNarrowGroups[1], Narrow<128, false, 2>::kPart) &&
-                  fits(kNarrowGroups[2], Narrow<128, false, 4>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
+static_assert(fits(1024, Narrow<64, false, 1>::kPart) && fits(768, Narrow<128, true, 1>::kPart) &&
+                  fits(512, Narrow<128, false, 2>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
               "partial results and tickets fit the workspace");
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
@@ -969,11 +1032,9 @@ static_assert(fits(kNarrowGroups[0], Narrow<128, false, 1>::kPart) && fits(kNarr
 template <int D, bool E4M3>
 void narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
   if (rows <= 16)
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kNarrowGroups[0]), dim3(kThreads), 0, stream, a);
-  else if (rows <= 32)
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kNarrowGroups[1]), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(narrow_groups<D, E4M3>(1)), dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 4>), dim3(kNarrowGroups[2]), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(narrow_groups<D, E4M3>(2)), dim3(kThreads), 0, stream, a);
 }
 
 template <int D, bool E4M3>
@@ -983,7 +1044,7 @@ void launch(PagedAttnArgs a, hipStream_t stream) {
   a.rows_max = INT32_MAX;
   if (rows <= 64) return narrow<D, E4M3>(a, rows, stream);
   // entries of a few rows beside longer ones: a launch of their own
-  const int few = a.group <= 16 ? 16 : a.group <= 32 ? 32 : 64;
+  const int few = a.group <= 16 ? 16 : 32;
   if (a.b.n > 1 && a.group <= few) {
     PagedAttnArgs b = a;
     b.rows_max = few;

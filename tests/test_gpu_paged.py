@@ -264,17 +264,19 @@ def test_attention_of_odd_batches(hk_lib):
     check_attention(*got, oracle.attention(cache.o, 0, _floats(q), seqs, first, 0.2), _floats(q), cache, 0.2)
 
 
-@pytest.mark.parametrize("dim,e4m3,counts", [(64, False, (1, 1)), (64, False, (4, 7)), (128, False, (90, 70)),
-                                             (128, True, (90, 1)), (64, True, (3, 130))])
-def test_attention_ignores_what_a_row_does_not_see(hk_lib, dim, e4m3, counts):
+@pytest.mark.parametrize("dim,e4m3,counts,window", [
+    (64, False, (1, 1), 60), (64, False, (4, 7), 60), (128, False, (90, 70), 60), (128, True, (90, 1), 60),
+    (64, True, (3, 130), 60), (64, False, (2, 3), 1500), (128, False, (100, 80), 1500), (128, True, (5, 90), 1500)])
+def test_attention_ignores_what_a_row_does_not_see(hk_lib, dim, e4m3, counts, window):
     """NaN and infinities in keys and values of later tokens, of slots left of the window, and behind the last slot."""
-    announce(f"paged attention: poisoned slots, dim {dim}, e4m3 {e4m3}, rows {counts}")
+    announce(f"paged attention: poisoned slots, dim {dim}, e4m3 {e4m3}, rows {counts}, window {window}")
     rng = np.random.default_rng(7)
-    cache = Cache(rng, pages=30, kv_heads=1, page=32, dim=dim, seqs=2, width=8, e4m3=e4m3)
-    cache.give([200, 147], rng)
+    lengths = [200, 147] if window < 100 else [2000, 1700]
+    cache = Cache(rng, pages=sum(lengths) // 32 + 4, kv_heads=1, page=32, dim=dim, seqs=2, width=lengths[0] // 32 + 1,
+                  e4m3=e4m3)
+    cache.give(lengths, rng)
     cache.fill(rng)
     bad = [np.nan] if e4m3 else [np.nan, np.inf, -np.inf]
-    window = 60
     for s, c in enumerate(counts):
         n = cache.o["length"][s]
         spots = [n - c - window, 0]  # left of every row's window
