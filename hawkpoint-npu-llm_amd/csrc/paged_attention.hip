@@ -304,14 +304,17 @@ __device__ __forceinline__ int v_key(int r) {
   return D == 128 ? 2 * (r & 7) : 2 * (((r >> 1) & 3) ^ (2 * (r & 1)));
 }
 
+// Workgroups per CU.
+constexpr int narrow_per_cu(int d, bool e4m3, int nq) { return nq == 2 ? 2 : d == 64 ? 4 : e4m3 ? 3 : 2; }
+
 template <int D, bool E4M3, int NQ>
-__global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_narrow_kernel(PagedAttnArgs a) {
   using N = Narrow<D, E4M3, NQ>;
   __shared__ __attribute__((aligned(16))) char lds[kWaves][N::kLds];
   __shared__ float wm[kWaves][N::kRows], wl[kWaves][N::kRows];
   __shared__ int last[2], again[kWaves];
-  constexpr int kJoin = 32;  // parts at a time
-  static_assert(2 * 4 * kJoin * N::kRows <= kWaves * N::kLds, "the weights fit the waves' LDS rows");
+  constexpr int kJoin = D * NQ == 256 ? 8 : 16;  // parts at a time
+  static_assert(4 * kJoin * N::kRows <= kWaves * N::kLds, "the weights fit the waves' LDS rows");
   const PlanShape shape = {a.c.kv_heads, a.group, a.window, N::kRows, kWaves * kNarrowSlots};
   const int w = run_of_group();
   Run run;
@@ -374,9 +377,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs
 
     u32x4 kr[2][N::kKLoads], vr[2][N::kVLoads];
     int there = 0, there_next = 0;  // bit h: slots 16 h .. of the tile have a page
+    int64_t at[2];
+    int bytes[2];
     // slots [s0, s0 + 32) of the tile, read through resources that end with the
     // page's rows below span.seen: later slots, and absent pages, read zero
-    auto load_tile = [&](int s0) {
+    auto find_tile = [&](int s0) {
       there_next = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -384,44 +389,37 @@ __global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs
         const int page = s < span.seen ? uniform(table[s >> shift]) : -1;
         const bool on = (unsigned)page < (unsigned)a.c.pages;
         if (on) there_next |= 1 << h;
-        const int bytes = on ? min(16, span.seen - s) * N::kRowBytes : 0;
-        const int64_t at = on ? page * a.c.page_bytes + (((int64_t)g << shift) + (s & mask)) * N::kRowBytes : 0;
-        const __amdgpu_buffer_rsrc_t kres = rsrc(a.c.k + at, bytes), vres = rsrc(a.c.v + at, bytes);
+        bytes[h] = on ? min(16, span.seen - s) * N::kRowBytes : 0;
+        at[h] = on ? page * a.c.page_bytes + (((int64_t)g << shift) + (s & mask)) * N::kRowBytes : 0;
+      }
+    };
+    auto load_v = [&]() {
 #pragma unroll
-        for (int i = 0; i < N::kKLoads; ++i)
-          kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(kres, col * N::kRowBytes + 16 * quad + 64 * i, 0, kStream);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < N::kVLoads; ++i)
-          vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, kStream);
-      }
+          vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.v + at[h], bytes[h]), 16 * lane + 1024 * i, 0, kStream);
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < N::kKLoads; ++i)
+          kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.k + at[h], bytes[h]),
+                                                           col * N::kRowBytes + 16 * quad + 64 * i, 0, kStream);
     };
 
     bool poison = false;
     const int s_end = min(kb1 * kWaves * kNarrowSlots, span.seen);
     int s0 = (kb0 * kWaves + wave) * kNarrowSlots;
-    if (s0 < s_end) load_tile(s0);
+    if (s0 < s_end) {
+      find_tile(s0);
+      load_v();
+      load_k();
+    }
     for (; s0 < s_end; s0 += kWaves * kNarrowSlots) {
       there = there_next;
-      // S^T: lane holds slots s0 + 16 h + 4 quad + r of row col
-      f32x4 sv[NQ][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) sv[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < N::kSteps; ++s) {
-          bf16x8 kf;
-          if constexpr (E4M3) {
-            const u32x4 raw = kr[h][s / 2];
-            const u32x2_t lo = e4m3_bf16(raw[2 * (s % 2)]), hi = e4m3_bf16(raw[2 * (s % 2) + 1]);
-            kf = __builtin_bit_cast(bf16x8, u32x4{lo.x, lo.y, hi.x, hi.y});
-          } else {
-            kf = __builtin_bit_cast(bf16x8, kr[h][s]);
-          }
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) sv[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][s], sv[n][h], 0, 0, 0);
-        }
-      }
+      const bool more = s0 + kWaves * kNarrowSlots < s_end;
       // V into LDS (the reads of the tile before are done: their values have
       // been used).  Where not every row sees every slot, an infinity or NaN
       // among the values is noted for rows_again.
@@ -447,7 +445,32 @@ __global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs
             if (!whole) bad |= not_finite(vr[h][i]);
           }
         }
-      if (s0 + kWaves * kNarrowSlots < s_end) load_tile(s0 + kWaves * kNarrowSlots);
+      // the next tile's loads go out as soon as their registers are free
+      if (more) {
+        find_tile(s0 + kWaves * kNarrowSlots);
+        load_v();
+      }
+      // S^T: lane holds slots s0 + 16 h + 4 quad + r of row col
+      f32x4 sv[NQ][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) sv[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < N::kSteps; ++s) {
+          bf16x8 kf;
+          if constexpr (E4M3) {
+            const u32x4 raw = kr[h][s / 2];
+            const u32x2_t lo = e4m3_bf16(raw[2 * (s % 2)]), hi = e4m3_bf16(raw[2 * (s % 2) + 1]);
+            kf = __builtin_bit_cast(bf16x8, u32x4{lo.x, lo.y, hi.x, hi.y});
+          } else {
+            kf = __builtin_bit_cast(bf16x8, kr[h][s]);
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) sv[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][s], sv[n][h], 0, 0, 0);
+        }
+      }
+      if (more) load_k();
 
       // a row sees slot s (no branches: the lanes differ)
       auto sees = [&](int n, int s) {
@@ -573,69 +596,74 @@ __global__ __launch_bounds__(kThreads, 2) void paged_narrow_kernel(PagedAttnArgs
   }
 
   const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
-  // joins a task's parts: their weights through LDS, 32 parts at a time, then
-  // four dimensions of a row per thread and step
-  float (&pm)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][0]);
-  float (&pl)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][sizeof(float) * kJoin * N::kRows]);
+  // joins a task's parts, kJoin at a time: all their loads go out at once, the
+  // maxima and sums give each row's weights of the parts (kRowThreads threads
+  // per row), and a thread adds up kItems words of four dimensions
+  constexpr int kQuads = D / 4, kItems = N::kRows * kQuads / kThreads, kRowThreads = kThreads / N::kRows;
+  float (&weight)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][0]);
   for (int j = 0; j < 2; ++j) {
     if (!((join >> j) & 1)) continue;
     const Pending& p = j ? pend[1] : pend[0];
     const PlanParts pp = plan_parts(p.start, p.units, run.per);
     const int r0 = p.tile * N::kRows, rows = min(N::kRows, p.entry.e.count * a.group - r0);
-    constexpr int kQuads = D / 4, kItems = N::kRows * kQuads / kThreads;
+    const int row = tid / kRowThreads, sub = tid % kRowThreads;
     f32x4 x[kItems] = {};
-    int note = 0;
-    __syncthreads();  // (wm, wl and the weights of another task have been read)
-    if (tid < N::kRows) wm[0][tid] = -INFINITY, wl[0][tid] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // of row `row`, in each of its threads
+    bool note = false;
     for (int k0 = 0; k0 < pp.count; k0 += kJoin) {
-      const int n = min(kJoin, pp.count - k0);
-      __syncthreads();
-      for (int i = tid; i < n * N::kRows; i += kThreads) {
-        const int k = i / N::kRows, r = i % N::kRows;
-        const int at = plan_slot(p.start, pp.first + k0 + k, run.per) * (N::kPart * 4);
-        pm[k][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * D + r), 0, kSc1));
-        pl[k][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * (D + 1) + r), 0, kSc1));
+      auto part = [&](int k) { return plan_slot(p.start, pp.first + min(k0 + k, pp.count - 1), run.per) * (N::kPart * 4); };
+      float pm[kJoin / kRowThreads], pl[kJoin / kRowThreads];
+      u32x4 y[kItems][kJoin];
+#pragma unroll
+      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+        const int at = part(sub + k * kRowThreads);
+        pm[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * D + row), 0, kSc1));
+        pl[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * (D + 1) + row), 0, kSc1));
       }
-      __syncthreads();
-      for (int k = 0; k < n; ++k) note |= pm[k][0] != pm[k][0];
-      __syncthreads();
-      if (tid < rows) {
-        const float m0 = wm[0][tid];
-        float m = m0;
-        for (int k = 0; k < n; ++k) m = fmaxf(m, pm[k][tid]);
-        const float f = __builtin_amdgcn_exp2f(m0 - finite_max(m));
-        float l = wl[0][tid] * f;
-        for (int k = 0; k < n; ++k) {
-          const float e = __builtin_amdgcn_exp2f(pm[k][tid] - finite_max(m));
-          l = fmaf(pl[k][tid], e, l);
-          pm[k][tid] = e;
-        }
-        wm[0][tid] = m, wl[0][tid] = l, wm[1][tid] = f;
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k)
+#pragma unroll
+        for (int i = 0; i < kItems; ++i)
+          y[i][k] = __builtin_amdgcn_raw_buffer_load_b128(parts, part(k) + 16 * (tid + i * kThreads), 0, kSc1);
+      float m_new = m;
+#pragma unroll
+      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+        m_new = fmaxf(m_new, pm[k]);
+        note |= pm[k] != pm[k];
       }
+      m_new = group_max<kRowThreads>(m_new);
+      const float f = __builtin_amdgcn_exp2f(m - finite_max(m_new));
+      float ls = 0.0f;
+      __syncthreads();  // (the weights before have been read)
+#pragma unroll
+      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+        const int i = sub + k * kRowThreads;
+        const float e = k0 + i < pp.count ? __builtin_amdgcn_exp2f(pm[k] - finite_max(m_new)) : 0.0f;
+        ls += k0 + i < pp.count ? pl[k] * e : 0.0f;
+        weight[i][row] = e;
+      }
+      l = l * f + group_sum<kRowThreads>(ls);
+      m = m_new;
+      if (sub == 0) wm[0][row] = m, wl[0][row] = l, wm[1][row] = f;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
-        const int r = (tid + i * kThreads) / kQuads, d = 4 * ((tid + i * kThreads) % kQuads);
-        if (r >= rows) break;
+        const int r = (tid + i * kThreads) / kQuads;
         x[i] *= wm[1][r];
-        constexpr int kBatch = 8;
-        for (int q = 0; q < n; q += kBatch) {
-          u32x4 y[kBatch];
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k)
-            y[k] = __builtin_amdgcn_raw_buffer_load_b128(
-                parts, plan_slot(p.start, pp.first + k0 + min(q + k, n - 1), run.per) * (N::kPart * 4) + 4 * (r * D + d), 0, kSc1);
+        for (int k = 0; k < kJoin; ++k) {
+          const float e = weight[k][r];
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            if (q + k >= n) break;
-            const float f = pm[q + k][r];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x[i][c] = fmaf(__uint_as_float(y[k][c]), f, x[i][c]);
-          }
+          for (int c = 0; c < 4; ++c) x[i][c] = k0 + k < pp.count ? fmaf(__uint_as_float(y[i][k][c]), e, x[i][c]) : x[i][c];
         }
       }
     }
-    if (note) {
+    // (a note is in the first row of a part, which is always there)
+    if (tid == 0) again[0] = 0;
+    __syncthreads();
+    if (row == 0 && note) again[0] = 1;
+    __syncthreads();
+    if (again[0]) {
       rows_again<D, E4M3>(a, p.entry, p.head, r0, rows);
       continue;
     }
@@ -1014,17 +1042,14 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
 }
 
 // Launches: as many workgroups as the GPU holds at once.
-template <int D, bool E4M3>
-constexpr int narrow_groups(int nq) {
-  return nq == 2 ? 512 : D == 64 ? 1024 : E4M3 ? 768 : 512;
-}
+constexpr int kCus = 256;
 constexpr int kWideQB = 1, kWideGroups = 512;
 constexpr bool fits(long long groups, long long part) {
   return groups <= kPagedTicketWords && groups % 8 == 0 &&
          4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
 }
-static_assert(fits(1024, Narrow<64, false, 1>::kPart) && fits(768, Narrow<128, true, 1>::kPart) &&
-                  fits(512, Narrow<128, false, 2>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
+static_assert(fits(4 * kCus, Narrow<64, false, 1>::kPart) && fits(3 * kCus, Narrow<128, true, 1>::kPart) &&
+                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
               "partial results and tickets fit the workspace");
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
@@ -1032,9 +1057,9 @@ static_assert(fits(1024, Narrow<64, false, 1>::kPart) && fits(768, Narrow<128, t
 template <int D, bool E4M3>
 void narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
   if (rows <= 16)
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(narrow_groups<D, E4M3>(1)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kCus * narrow_per_cu(D, E4M3, 1)), dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(narrow_groups<D, E4M3>(2)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kCus * narrow_per_cu(D, E4M3, 2)), dim3(kThreads), 0, stream, a);
 }
 
 template <int D, bool E4M3>
