@@ -19,6 +19,8 @@
 // and there is nothing to plan between the calls.  A task that is cut leaves
 // (max, sum, O) of its parts in the workspace, and the workgroup that arrives
 // last (a ticket per task, zero between launches) joins them in their order.
+#include <type_traits>
+
 #include "hk_common.h"
 #include "hk_internal.h"
 #include "paged.h"
@@ -43,6 +45,13 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
   return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The load of v is waited for here.
+__device__ __forceinline__ void settle(bf16x8& v) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(v));
+#endif
 }
 
 // A table entry at a uniform place, through the scalar cache: a vector load
@@ -156,8 +165,8 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
       seq = entry_seq(a.c, a.b, b);
     }
     const PlanEntry e = {seq.y, rows.y - rows.x};
-    const bool has = b < n && takes(a, e.count), few = has && e.count * s.group <= s.rows;
-    int64_t u = few ? (int64_t)s.heads * plan_units(plan_span(s, e, 0)) : 0;
+    const bool has = b < n && takes(a, e.count), few = has && e.count * s.group <= 4 * s.rows;
+    int64_t u = few ? s.heads * plan_head_units(s, e) : 0;
     // entries of more tiles: the wave's lanes together
     for (unsigned long long todo = __ballot(has && !few); todo; todo &= todo - 1) {
       const int l = __builtin_ctzll(todo);
@@ -219,6 +228,33 @@ __device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShap
     run.entry = load_entry(a, p.entry);
     if (takes(a, run.entry.e.count)) return;
   }
+}
+
+// A workgroup's part of a task: blocks [kb0, kb1) of the `rows` rows from r0 of
+// kv head g, of which it sees slots below `seen`.
+struct Task {
+  Entry entry;
+  const int32_t* table;  // the sequence's pages
+  int64_t start;         // units before the task
+  int g, tile, r0, rows, pos0, units, take, kb0, kb1, seen;
+};
+__device__ __forceinline__ Task task_of(const PagedAttnArgs& a, const PlanShape& s, const Run& run) {
+  Task t;
+  const PlanSpan span = plan_span(s, run.entry.e, run.place.tile);
+  t.entry = run.entry;
+  t.table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
+  t.start = run.place.start;
+  t.g = run.place.head;
+  t.tile = run.place.tile;
+  t.r0 = run.place.tile * s.rows;
+  t.rows = min(s.rows, run.entry.e.count * a.group - t.r0);
+  t.pos0 = run.entry.e.length - run.entry.e.count;
+  t.units = plan_units(span);
+  t.take = (int)min((int64_t)(t.units - run.place.at), run.end - run.unit);
+  t.kb0 = span.lo + run.place.at;
+  t.kb1 = span.hi > span.lo ? t.kb0 + t.take : t.kb0;
+  t.seen = span.seen;
+  return t;
 }
 
 // Consecutive runs on one XCD (workgroups go round the eight XCDs), where they
@@ -396,15 +432,61 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     if (a.lse && d == 0) stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2);
   };
 
-  while (run.unit < run.end) {
-    const PlanSpan span = plan_span(shape, run.entry.e, run.place.tile);
-    const int units = plan_units(span);
-    const int take = (int)min((int64_t)(units - run.place.at), run.end - run.unit);
-    const int g = run.place.head, r0 = run.place.tile * N::kRows;
-    const int rows = min(N::kRows, run.entry.e.count * a.group - r0);
-    const int pos0 = run.entry.e.length - run.entry.e.count;
-    const int kb0 = span.lo + run.place.at, kb1 = span.hi > span.lo ? kb0 + take : kb0;
-    const int32_t* const table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
+  u32x4 kr[2][N::kKLoads], vr[2][N::kVLoads];
+  int there = 0, there_next = 0;  // bit h: slots 16 h .. of the tile have a page
+  int64_t at[2];
+  int bytes[2], page[2];
+  // the tile's pages, asked for a tile before their rows
+  auto find_pages = [&](const Task& t, int s0) {
+    const int s_end = min(t.kb1 * kWaves * kNarrowSlots, t.seen);
+
+#pragma unroll
+    for (int h = 0; h < 2; ++h) page[h] = s0 + 16 * h < s_end ? table_at(t.table, (s0 + 16 * h) >> shift) : -1;
+  };
+  // slots [s0, s0 + 32) of the tile, read through resources that end with the
+  // page's rows below t.seen: later slots, and absent pages, read zero
+  auto find_tile = [&](const Task& t, int s0) {
+    there_next = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int s = s0 + 16 * h;
+      const bool on = (unsigned)page[h] < (unsigned)a.c.pages;
+      if (on) there_next |= 1 << h;
+      bytes[h] = on ? min(16, t.seen - s) * N::kRowBytes : 0;
+      at[h] = on ? page[h] * a.c.page_bytes + (((int64_t)t.g << shift) + (s & mask)) * N::kRowBytes : 0;
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < N::kVLoads; ++i)
+        vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.v + at[h], bytes[h]), 16 * lane + 1024 * i, 0, kStream);
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < N::kKLoads; ++i)
+        kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.k + at[h], bytes[h]),
+                                                         col * N::kRowBytes + 16 * quad + 64 * i, 0, kStream);
+  };
+
+  // the first loads of a task
+  auto begin = [&](const Task& t) {
+    const int s0 = (t.kb0 * kWaves + wave) * kNarrowSlots;
+    if (s0 >= min(t.kb1 * kWaves * kNarrowSlots, t.seen)) return;
+    find_pages(t, s0);
+    find_tile(t, s0);
+    load_v();
+    load_k();
+    find_pages(t, s0 + kWaves * kNarrowSlots);
+  };
+
+  Task t = task_of(a, shape, run);
+  begin(t);
+  for (;;) {
+    const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g;
     const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
 
     // this lane's rows: position, and Q as the right operand (row col of each
@@ -417,13 +499,19 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       const bool ok = 16 * n + col < rows;
       pos[n] = ok ? pos0 + tok : -1;
       low[n] = a.window > 0 ? pos[n] - a.window : -1;
-      const uint16_t* q = a.q + (run.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
+      const uint16_t* q = a.q + (t.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
 #pragma unroll
       for (int s = 0; s < N::kSteps; ++s) {
         const int d = E4M3 ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 32 * s + 8 * quad;
         qf[n][s] = __builtin_bit_cast(bf16x8, load16(q + d));
       }
     }
+    // Q is there before the loop: a wait inside it would be one for the K and V
+    // loads in flight too
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int s = 0; s < N::kSteps; ++s) settle(qf[n][s]);
 
     float m_run[NQ], l_run[NQ];
     f32x4 o[NQ][N::kDims];
@@ -435,55 +523,9 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       for (int d = 0; d < N::kDims; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    u32x4 kr[2][N::kKLoads], vr[2][N::kVLoads];
-    int there = 0, there_next = 0;  // bit h: slots 16 h .. of the tile have a page
-    int64_t at[2];
-    int bytes[2], page[2];
-    const int s_end = min(kb1 * kWaves * kNarrowSlots, span.seen);
-    // the tile's pages, asked for a tile before their rows
-    auto find_pages = [&](int s0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = s0 + 16 * h < s_end ? table_at(table, (s0 + 16 * h) >> shift) : -1;
-    };
-    // slots [s0, s0 + 32) of the tile, read through resources that end with the
-    // page's rows below span.seen: later slots, and absent pages, read zero
-    auto find_tile = [&](int s0) {
-      there_next = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int s = s0 + 16 * h;
-        const bool on = (unsigned)page[h] < (unsigned)a.c.pages;
-        if (on) there_next |= 1 << h;
-        bytes[h] = on ? min(16, span.seen - s) * N::kRowBytes : 0;
-        at[h] = on ? page[h] * a.c.page_bytes + (((int64_t)g << shift) + (s & mask)) * N::kRowBytes : 0;
-      }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < N::kVLoads; ++i)
-          vr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.v + at[h], bytes[h]), 16 * lane + 1024 * i, 0, kStream);
-    };
-    auto load_k = [&]() {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < N::kKLoads; ++i)
-          kr[h][i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.c.k + at[h], bytes[h]),
-                                                           col * N::kRowBytes + 16 * quad + 64 * i, 0, kStream);
-    };
-
     bool poison = false;
-    int s0 = (kb0 * kWaves + wave) * kNarrowSlots;
-    if (s0 < s_end) {
-      find_pages(s0);
-      find_tile(s0);
-      load_v();
-      load_k();
-      find_pages(s0 + kWaves * kNarrowSlots);
-    }
-    for (; s0 < s_end; s0 += kWaves * kNarrowSlots) {
+    const int s_end = min(t.kb1 * kWaves * kNarrowSlots, t.seen);
+    for (int s0 = (t.kb0 * kWaves + wave) * kNarrowSlots; s0 < s_end; s0 += kWaves * kNarrowSlots) {
       there = there_next;
       const bool more = s0 + kWaves * kNarrowSlots < s_end;
       // V into LDS (the reads of the tile before are done: their values have
@@ -513,9 +555,9 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
         }
       // the next tile's loads go out as soon as their registers are free
       if (more) {
-        find_tile(s0 + kWaves * kNarrowSlots);
+        find_tile(t, s0 + kWaves * kNarrowSlots);
         load_v();
-        find_pages(s0 + 2 * kWaves * kNarrowSlots);
+        find_pages(t, s0 + 2 * kWaves * kNarrowSlots);
       }
       // S^T: lane holds slots s0 + 16 h + 4 quad + r of row col
       f32x4 sv[NQ][2];
@@ -593,6 +635,16 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       }
     }
 
+    // the next task's first loads are under way while this one ends
+    const Task done = t;
+    run.unit += t.take;
+    const bool more_tasks = run.unit < run.end;
+    if (more_tasks) {
+      plan_next(a, shape, run, t.units);
+      t = task_of(a, shape, run);
+      begin(t);
+    }
+
     // the waves' results meet: maxima and sums, then O through LDS 16 rows at a time
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -606,8 +658,8 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       const int any = __any(poison);
       if (lane == 0) again[wave] = any;
     }
-    const bool cut = take < units;
-    const int slot = plan_slot(run.place.start, w, run.per) * (N::kPart * 4);
+    const bool cut = done.take < done.units;
+    const int slot = plan_slot(done.start, w, run.per) * (N::kPart * 4);
     constexpr int kPer = D / 16;  // outputs of a thread: dimensions kPer (tid % 16) .. of row tid / 16
     const int orow = tid >> 4, od = kPer * (tid & 15);
     bool note = false;
@@ -643,7 +695,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
         if (cut)
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, slot + 4 * (r * D + od + i), 0, kSc1);
         else if (!note)
-          finish(run.entry, g, r0 + r, od + i, y, m, l);
+          finish(done.entry, g, r0 + r, od + i, y, m, l);
       }
       if (cut && (tid & 15) == 0) {
         // (a NaN in the place of a maximum, which none is, passes the note on)
@@ -652,49 +704,47 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       }
     }
     __syncthreads();  // the waves' V rows are free again
-    if (!cut && note) rows_again<D, E4M3>(a, run.entry, g, r0, rows);
+    if (!cut && note) rows_again<D, E4M3>(a, done.entry, g, r0, rows);
     if (cut) {
-      const Pending p = {run.place.start, run.entry, units, g, run.place.tile};
+      const Pending p = {done.start, done.entry, done.units, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     }
-    run.unit += take;
-    if (run.unit < run.end) plan_next(a, shape, run, units);
+    if (!more_tasks) break;
   }
 
   const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
-  // joins a task's parts, kJoin at a time: all their loads go out at once, the
+  // joins a task's parts, J at a time: all their loads go out at once, the
   // maxima and sums give each row's weights of the parts (kRowThreads threads
   // per row), and a thread adds up kItems words of four dimensions
   constexpr int kQuads = D / 4, kItems = N::kRows * kQuads / kThreads, kRowThreads = kThreads / N::kRows;
   float (&weight)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][0]);
-  for (int j = 0; j < 2; ++j) {
-    if (!((join >> j) & 1)) continue;
-    const Pending& p = j ? pend[1] : pend[0];
+  auto join_task = [&](const Pending& p, auto steps) {
+    constexpr int J = decltype(steps)::value, kMine = (J + kRowThreads - 1) / kRowThreads;
     const PlanParts pp = plan_parts(p.start, p.units, run.per);
     const int r0 = p.tile * N::kRows, rows = min(N::kRows, p.entry.e.count * a.group - r0);
     const int row = tid / kRowThreads, sub = tid % kRowThreads;
     f32x4 x[kItems] = {};
     float m = -INFINITY, l = 0.0f;  // of row `row`, in each of its threads
     bool note = false;
-    for (int k0 = 0; k0 < pp.count; k0 += kJoin) {
+    for (int k0 = 0; k0 < pp.count; k0 += J) {
       auto part = [&](int k) { return plan_slot(p.start, pp.first + min(k0 + k, pp.count - 1), run.per) * (N::kPart * 4); };
-      float pm[kJoin / kRowThreads], pl[kJoin / kRowThreads];
-      u32x4 y[kItems][kJoin];
+      float pm[kMine], pl[kMine];
+      u32x4 y[kItems][J];
 #pragma unroll
-      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+      for (int k = 0; k < kMine; ++k) {
         const int at = part(sub + k * kRowThreads);
         pm[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * D + row), 0, kSc1));
         pl[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * (D + 1) + row), 0, kSc1));
       }
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k)
+      for (int k = 0; k < J; ++k)
 #pragma unroll
         for (int i = 0; i < kItems; ++i)
           y[i][k] = __builtin_amdgcn_raw_buffer_load_b128(parts, part(k) + 16 * (tid + i * kThreads), 0, kSc1);
       float m_new = m;
 #pragma unroll
-      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+      for (int k = 0; k < kMine; ++k) {
         m_new = fmaxf(m_new, pm[k]);
         note |= pm[k] != pm[k];
       }
@@ -703,11 +753,12 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       float ls = 0.0f;
       __syncthreads();  // (the weights before have been read)
 #pragma unroll
-      for (int k = 0; k < kJoin / kRowThreads; ++k) {
+      for (int k = 0; k < kMine; ++k) {
         const int i = sub + k * kRowThreads;
-        const float e = k0 + i < pp.count ? __builtin_amdgcn_exp2f(pm[k] - finite_max(m_new)) : 0.0f;
-        ls += k0 + i < pp.count ? pl[k] * e : 0.0f;
-        weight[i][row] = e;
+        const bool on = i < J && k0 + i < pp.count;
+        const float e = on ? __builtin_amdgcn_exp2f(pm[k] - finite_max(m_new)) : 0.0f;
+        ls += on ? pl[k] * e : 0.0f;
+        if (i < J) weight[i][row] = e;
       }
       l = l * f + group_sum<kRowThreads>(ls);
       m = m_new;
@@ -718,7 +769,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
         const int r = (tid + i * kThreads) / kQuads;
         x[i] *= wm[1][r];
 #pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
+        for (int k = 0; k < J; ++k) {
           const float e = weight[k][r];
 #pragma unroll
           for (int c = 0; c < 4; ++c) x[i][c] = k0 + k < pp.count ? fmaf(__uint_as_float(y[i][k][c]), e, x[i][c]) : x[i][c];
@@ -732,13 +783,22 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     __syncthreads();
     if (again[0]) {
       rows_again<D, E4M3>(a, p.entry, p.head, r0, rows);
-      continue;
+      return;
     }
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int r = (tid + i * kThreads) / kQuads, d = 4 * ((tid + i * kThreads) % kQuads);
       if (r < rows) finish(p.entry, p.head, r0 + r, d, x[i], wm[0][r], wl[0][r]);
     }
+  };
+  for (int j = 0; j < 2; ++j) {
+    if (!((join >> j) & 1)) continue;
+    const Pending& p = j ? pend[1] : pend[0];
+    __syncthreads();  // (wm and wl of another task have been read)
+    if (plan_parts(p.start, p.units, run.per).count <= 4)
+      join_task(p, std::integral_constant<int, 4>());
+    else
+      join_task(p, std::integral_constant<int, kJoin>());
   }
 }
 
@@ -782,10 +842,13 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+constexpr int wide_per_cu(int d) { return d == 64 ? 3 : 2; }
+
 template <int D, bool E4M3, int QB>
-__global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(PagedAttnArgs a) {
   using W = Wide<D, QB>;
   constexpr int kRowBytes = D * (E4M3 ? 1 : 2), kLoads = kRowBytes / 64, kSteps = D / 16, kDims = D / 32;
+  constexpr int kAhead = 2;
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
   // of each 16 slots of a block: bit 0: they have a page, bit 1: an infinity or
@@ -827,15 +890,38 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
     }
   };
 
-  while (run.unit < run.end) {
-    const PlanSpan span = plan_span(shape, run.entry.e, run.place.tile);
-    const int units = plan_units(span);
-    const int take = (int)min((int64_t)(units - run.place.at), run.end - run.unit);
-    const int g = run.place.head, r0 = run.place.tile * W::kRows;
-    const int rows = min(W::kRows, run.entry.e.count * a.group - r0);
-    const int pos0 = run.entry.e.length - run.entry.e.count;
-    const int kb0 = span.lo + run.place.at, kb1 = span.hi > span.lo ? kb0 + take : kb0;
-    const int32_t* const table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
+  // wave w loads slots 16 w .. of a block (one page's): resources that end
+  // with the rows below t.seen, so later slots and absent pages read zero
+  u32x4 kr[kLoads], vr[kLoads];
+  int page, there;
+  auto find_page = [&](const Task& t, int s0) {  // asked for a block before its rows
+    const int s = s0 + 16 * wave;
+    page = s < t.seen ? table_at(t.table, s >> shift) : -1;
+  };
+  auto load_block = [&](const Task& t, int s0) {
+    const int s = s0 + 16 * wave;
+    const bool on = (unsigned)page < (unsigned)a.c.pages;
+    there = on;
+    const int bytes = on ? min(16, t.seen - s) * kRowBytes : 0;
+    const int64_t at = on ? page * a.c.page_bytes + (((int64_t)t.g << shift) + (s & mask)) * kRowBytes : 0;
+    const __amdgpu_buffer_rsrc_t kres = rsrc(a.c.k + at, bytes), vres = rsrc(a.c.v + at, bytes);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kres, 16 * lane + 1024 * i, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, 0);
+  };
+  // the first loads of a task
+  auto begin = [&](const Task& t) {
+    if (t.kb0 >= t.kb1) return;
+    find_page(t, t.kb0 * kWideSlots);
+    load_block(t, t.kb0 * kWideSlots);
+    find_page(t, (t.kb0 + 1) * kWideSlots);
+  };
+
+  Task t = task_of(a, shape, run);
+  begin(t);
+  for (;;) {
+    const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g, kb0 = t.kb0, kb1 = t.kb1;
     const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
     // the wave's rows [w0, w1) of the tile, and the positions they span
     const int w0 = wave * 32 * QB, w1 = min(rows, w0 + 32 * QB);
@@ -850,10 +936,14 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
       const bool ok = at < rows;
       pos[b] = ok ? pos0 + tok : -1;
       low[b] = a.window > 0 ? pos[b] - a.window : -1;
-      const uint16_t* q = a.q + (run.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
+      const uint16_t* q = a.q + (t.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) qf[b][s] = __builtin_bit_cast(bf16x8, load16(q + 16 * s + 8 * half));
     }
+#pragma unroll
+    for (int b = 0; b < QB; ++b)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) settle(qf[b][s]);  // (before the loop, as in the narrow form)
     float m_run[QB], l_run[QB];
     f32x16 o[QB][kDims];
 #pragma unroll
@@ -866,26 +956,6 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
         for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
     }
 
-    // wave w loads slots 16 w .. of a block (one page's): resources that end
-    // with the rows below span.seen, so later slots and absent pages read zero
-    u32x4 kr[kLoads], vr[kLoads];
-    int page, there;
-    auto find_page = [&](int s0) {  // asked for a block before its rows
-      const int s = s0 + 16 * wave;
-      page = s < span.seen ? table_at(table, s >> shift) : -1;
-    };
-    auto load_block = [&](int s0) {
-      const int s = s0 + 16 * wave;
-      const bool on = (unsigned)page < (unsigned)a.c.pages;
-      there = on;
-      const int bytes = on ? min(16, span.seen - s) * kRowBytes : 0;
-      const int64_t at = on ? page * a.c.page_bytes + (((int64_t)g << shift) + (s & mask)) * kRowBytes : 0;
-      const __amdgpu_buffer_rsrc_t kres = rsrc(a.c.k + at, bytes), vres = rsrc(a.c.v + at, bytes);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kres, 16 * lane + 1024 * i, 0, 0);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vres, 16 * lane + 1024 * i, 0, 0);
-    };
     // a block that every row of the tile sees whole (its pages apart)
     auto all_see = [&](int s0, int lo, int hi) {
       return s0 + kWideSlots - 1 <= lo && (a.window == 0 || s0 > hi - a.window);
@@ -918,35 +988,44 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
     };
 
     int poison = 0;  // an infinity or NaN among values that not every row sees, for rows_again
-    if (kb0 < kb1) {
-      find_page(kb0 * kWideSlots);
-      load_block(kb0 * kWideSlots);
-      find_page((kb0 + 1) * kWideSlots);
-      store_block(kb0 * kWideSlots, 0);
-    }
+    if (kb0 < kb1) store_block(kb0 * kWideSlots, 0);
     for (int kb = kb0, buf = 0; kb < kb1; ++kb, buf ^= 1) {
       const int s0 = kb * kWideSlots;
       __syncthreads();  // the block is there, and the other buffer has been read
-      if (kb + 1 < kb1) {
-        load_block(s0 + kWideSlots);
-        find_page(s0 + 2 * kWideSlots);
-      }
+      if (kb + 1 < kb1) load_block(t, s0 + kWideSlots);
       if (s0 <= wave_hi) {
         const u32x4 notes = *reinterpret_cast<const u32x4*>(note_lds[buf]);
-        // S^T: lane holds slots 32 t + 8 (i / 4) + 4 half + i % 4 of row col
+        // S^T: lane holds slots 32 t + 8 (i / 4) + 4 half + i % 4 of row col.  The
+        // fragments of kAhead products are read while those before them run
+        // (left to itself the compiler reads one and waits for it)
         f32x16 sv[QB][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int b = 0; b < QB; ++b)
 #pragma unroll
-          for (int b = 0; b < QB; ++b)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sv[b][t][i] = 0.0f;
-          const int r = 32 * t + col;
+        {
+          bf16x8 kf[2][kAhead];
+          auto read_k = [&](int x) {  // fragments kAhead x ..: step % kSteps of slots 32 (step / kSteps) ..
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&ks_lds[buf][r * D + 8 * ((2 * s + half) ^ wide_k_key<D>(r))]);
+            for (int y = 0; y < kAhead; ++y) {
+              const int r = 32 * ((kAhead * x + y) / kSteps) + col, s = (kAhead * x + y) % kSteps;
+              kf[x & 1][y] = *reinterpret_cast<const bf16x8*>(&ks_lds[buf][r * D + 8 * ((2 * s + half) ^ wide_k_key<D>(r))]);
+            }
+          };
+          read_k(0);
 #pragma unroll
-            for (int b = 0; b < QB; ++b) sv[b][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[b][s], sv[b][t], 0, 0, 0);
+          for (int x = 0; x < 2 * kSteps / kAhead; ++x) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (x + 1 < 2 * kSteps / kAhead) read_k(x + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < kAhead; ++y)
+#pragma unroll
+              for (int b = 0; b < QB; ++b)
+                sv[b][(kAhead * x + y) / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    kf[x & 1][y], qf[b][(kAhead * x + y) % kSteps], sv[b][(kAhead * x + y) / kSteps], 0, 0, 0);
           }
         }
         // bit h: slots 16 h .. of the block have a page
@@ -1003,26 +1082,52 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
           // 4 half + e % 4, the probabilities this lane holds; a group of 16
           // lanes reads 4 slots of 16 dimensions, transposed
           const int ra = 4 * half + ((lane & 15) >> 2), dd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          bf16x8 vf[2][kAhead];
+          auto read_v = [&](int x) {  // fragments kAhead x ..: dimensions 32 (step % kDims) .. of slots 16 (step / kDims) ..
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) {
+            for (int y = 0; y < kAhead; ++y) {
+              const int t = (kAhead * x + y) / kDims, d = (kAhead * x + y) % kDims;
               const int r1 = 16 * t + ra, r2 = r1 + 8, dim = 32 * d + dd;
               const v4s16 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                   (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r1 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r1)) + (dim & 7)]);
               const v4s16 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                   (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r2 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r2)) + (dim & 7)]);
               const u32x2_t w0 = __builtin_bit_cast(u32x2_t, t0), w1 = __builtin_bit_cast(u32x2_t, t1);
-              const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{w0.x, w0.y, w1.x, w1.y});
-#pragma unroll
-              for (int b = 0; b < QB; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[b][t], o[b][d], 0, 0, 0);
+              vf[x & 1][y] = __builtin_bit_cast(bf16x8, u32x4{w0.x, w0.y, w1.x, w1.y});
             }
+          };
+          read_v(0);
+#pragma unroll
+          for (int x = 0; x < 4 * kDims / kAhead; ++x) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (x + 1 < 4 * kDims / kAhead) read_v(x + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < kAhead; ++y) {
+              const int t = (kAhead * x + y) / kDims, d = (kAhead * x + y) % kDims;
+#pragma unroll
+              for (int b = 0; b < QB; ++b)
+                o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 1][y], pf[b][t], o[b][d], 0, 0, 0);
+            }
+          }
         }
       }
-      if (kb + 1 < kb1) store_block(s0 + kWideSlots, buf ^ 1);
+      if (kb + 1 < kb1) {
+        find_page(t, s0 + 2 * kWideSlots);
+        store_block(s0 + kWideSlots, buf ^ 1);
+      }
     }
 
-    const bool cut = take < units;
+    // the next task's first loads are under way while this one ends
+    const Task done = t;
+    run.unit += t.take;
+    const bool more_tasks = run.unit < run.end;
+    if (more_tasks) {
+      plan_next(a, shape, run, t.units);
+      t = task_of(a, shape, run);
+      begin(t);
+    }
+    const bool cut = done.take < done.units;
 #pragma unroll
     for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
     if (lane == 0) again[wave] = poison;
@@ -1030,7 +1135,7 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
     const bool note = again[0] | again[1] | again[2] | again[3];
     if (cut) {
       // parts lie lane by lane: word i of thread t at 16 (i threads + t) bytes
-      const int slot = plan_slot(run.place.start, w, run.per) * (W::kPart * 4);
+      const int slot = plan_slot(done.start, w, run.per) * (W::kPart * 4);
       if (wave_hi >= 0) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
@@ -1046,17 +1151,16 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
                                                 slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
         }
       }
-      const Pending p = {run.place.start, run.entry, units, g, run.place.tile};
+      const Pending p = {done.start, done.entry, done.units, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     } else if (note) {
-      rows_again<D, E4M3>(a, run.entry, g, r0, rows);
+      rows_again<D, E4M3>(a, done.entry, g, r0, rows);
     } else {
-      finish(run.entry, g, r0, rows, o, m_run, l_run);
+      finish(done.entry, g, r0, rows, o, m_run, l_run);
     }
     __syncthreads();  // (the notes have been read)
-    run.unit += take;
-    if (run.unit < run.end) plan_next(a, shape, run, units);
+    if (!more_tasks) break;
   }
 
   const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
@@ -1113,13 +1217,14 @@ __global__ __launch_bounds__(kThreads, QB == 1 ? 2 : 1) void paged_wide_kernel(P
 
 // Launches: as many workgroups as the GPU holds at once.
 constexpr int kCus = 256;
-constexpr int kWideQB = 1, kWideGroups = 512;
+constexpr int kWideQB = 1;
 constexpr bool fits(long long groups, long long part) {
   return groups <= kPagedTicketWords && groups % 8 == 0 &&
          4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
 }
 static_assert(fits(4 * kCus, Narrow<64, false, 1>::kPart) && fits(3 * kCus, Narrow<128, true, 1>::kPart) &&
-                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kWideGroups, Wide<128, kWideQB>::kPart),
+                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kCus * wide_per_cu(128), Wide<128, kWideQB>::kPart) &&
+                  fits(kCus * wide_per_cu(64), Wide<64, kWideQB>::kPart),
               "partial results and tickets fit the workspace");
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
@@ -1146,7 +1251,7 @@ void launch(PagedAttnArgs a, hipStream_t stream) {
     a.rows_min = few + 1;
     narrow<D, E4M3>(b, few, stream);
   }
-  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3, kWideQB>), dim3(kWideGroups), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3, kWideQB>), dim3(kCus * wide_per_cu(D)), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
