@@ -40,6 +40,7 @@ constexpr int kWaves = kThreads / 64;
 // buffer access cache policies
 constexpr int kSc1 = 16;    // device scope
 constexpr int kStream = 2;  // read once: does not stay in the caches
+constexpr int kNowhere = 0x7ffffff0;  // an offset past any resource: reads zero, no memory access
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -115,11 +116,16 @@ __device__ __forceinline__ int64_t wave_head_units(const PlanShape& s, const Pla
   return uniform(n);
 }
 __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
-  const int lane = threadIdx.x & 63;
-  const int64_t per_head = wave_head_units(s, e);
-  PlanPlace p = {entry, uniform((int)(rem / per_head)), 0, 0, 0};
+  const int lane = threadIdx.x & 63, tiles = plan_tiles(s, e);
+  const int64_t per_head = tiles == 1 ? plan_units(plan_span(s, e, 0)) : wave_head_units(s, e);
+  PlanPlace p = {entry, uniform((int)plan_div(rem, per_head)), 0, 0, 0};
   rem -= p.head * per_head;
   start += p.head * per_head;
+  if (tiles == 1) {
+    p.at = (int)rem;
+    p.start = start;
+    return p;
+  }
   for (;; p.tile += 64) {
     const int u = wave_units(s, e, p.tile + lane);
     int64_t sum = u;
@@ -129,7 +135,7 @@ __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEnt
       if (lane >= m) sum += v;
     }
     const unsigned long long past = __ballot(sum > rem);
-    if (past == 0 && p.tile + 64 < plan_tiles(s, e)) {
+    if (past == 0 && p.tile + 64 < tiles) {
       const int64_t all = uniform(__shfl(sum, 63, 64));
       rem -= all;
       start += all;
@@ -734,6 +740,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
         const int at = part(sub + k * kRowThreads);
+        // (of rows that the task has not, words that nobody wrote: not used)
         pm[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * D + row), 0, kSc1));
         pl[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at + 4 * (N::kRows * (D + 1) + row), 0, kSc1));
       }
@@ -741,7 +748,8 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       for (int k = 0; k < J; ++k)
 #pragma unroll
         for (int i = 0; i < kItems; ++i)
-          y[i][k] = __builtin_amdgcn_raw_buffer_load_b128(parts, part(k) + 16 * (tid + i * kThreads), 0, kSc1);
+          y[i][k] = __builtin_amdgcn_raw_buffer_load_b128(
+              parts, (tid + i * kThreads) / kQuads < rows ? part(k) + 16 * (tid + i * kThreads) : kNowhere, 0, kSc1);
       float m_new = m;
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {

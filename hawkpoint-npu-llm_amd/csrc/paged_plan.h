@@ -56,8 +56,14 @@ HK_PLAN int64_t plan_head_units(const PlanShape& s, const PlanEntry& e) {
   return n;
 }
 
+// a / b of numbers that are not negative, in 32 bits where they fit (on the GPU
+// a 64-bit division costs four times as much).
+HK_PLAN int64_t plan_div(int64_t a, int64_t b) {
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 HK_PLAN int64_t plan_per(int64_t total, int groups, int least) {
-  const int64_t per = (total + groups - 1) / groups;
+  const int64_t per = plan_div(total + groups - 1, groups);
   return per > least ? per : least;
 }
 
@@ -72,7 +78,7 @@ struct PlanPlace {
 // The place `rem` units into entry `entry`, which starts at unit `start`.
 HK_PLAN PlanPlace plan_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
   const int64_t per_head = plan_head_units(s, e);
-  PlanPlace p = {entry, (int)(rem / per_head), 0, 0, 0};
+  PlanPlace p = {entry, (int)plan_div(rem, per_head), 0, 0, 0};
   rem -= p.head * per_head;
   start += p.head * per_head;
   for (;;) {
@@ -94,7 +100,7 @@ struct PlanParts {
   int first, count;
 };
 HK_PLAN PlanParts plan_parts(int64_t start, int units, int64_t per) {
-  const int first = (int)(start / per), last = (int)((start + units - 1) / per);
+  const int first = (int)plan_div(start, per), last = (int)plan_div(start + units - 1, per);
   return {first, last - first + 1};
 }
 HK_PLAN int plan_slot(int64_t start, int w, int64_t per) { return 2 * w + (start >= w * per ? 1 : 0); }
