@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "hk_paged.h"
+#include "paged_plan.h"
 
 namespace hk {
 
@@ -38,6 +39,7 @@ struct PagedAttnArgs {
   float* lse;
   int64_t q_stride, out_stride;
   int q_heads, group, window, max_new;
+  PlanDivisor by_group;    // set by the launch
   int rows_min, rows_max;  // set by the launch: rows (tokens x group) of the entries it takes
   float scale;
   void* workspace;

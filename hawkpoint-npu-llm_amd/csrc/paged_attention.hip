@@ -63,13 +63,24 @@ __device__ __forceinline__ int table_at(const int32_t* table, int i) {
 
 // ---- a workgroup's run of the work ----
 
+// What a task costs beside its blocks: its first loads' latency, its end and,
+// for a cut one, the workspace, in halves of a block.  Without it the
+// workgroups that have many short tasks end last (190 chats: 69 us against 64,
+// pieces of prompts beside chats 72 and 62; one half more or less is the same).
+constexpr int kBlockCost = 2, kNarrowTaskCost = 3, kWideTaskCost = 3;
+
 struct Entry {
   int seq, row0;  // sequence (-1: none), first row
   PlanEntry e;
 };
+// Entry b (uniform), through the scalar cache: entry_rows and entry_seq.
 __device__ __forceinline__ Entry load_entry(const PagedAttnArgs& a, int b) {
-  const int2 r = entry_rows(a.b, b), s = entry_seq(a.c, a.b, b);
-  return {uniform(s.x), uniform(r.x), {uniform(s.y), uniform(r.y - r.x)}};
+  const int f0 = min(max(table_at(a.b.first, b), 0), a.b.tokens);
+  const int f1 = min(max(table_at(a.b.first, b + 1), f0), a.b.tokens);
+  const int s = a.b.seqs ? table_at(a.b.seqs, b) : b;
+  const bool is = (unsigned)s < (unsigned)a.c.seqs;
+  const int length = is ? min(max(table_at(a.c.length, s), 0), a.c.width << a.c.page_shift) : 0;
+  return {is ? s : -1, f0, {length, f1 - f0}};
 }
 
 // Whether an entry of `count` rows is this launch's (a batch of long and short
@@ -104,30 +115,27 @@ __device__ __forceinline__ int64_t scan(int64_t v, int64_t* sums, int64_t& total
 // plan_head_units and plan_find (paged_plan.h), a wave's lanes taking 64 tiles
 // at a time: one thread that walked the tiles of a prompt's piece took 12 us
 // for 701 tokens and 32 us for 2039.  The arguments are uniform.
-__device__ __forceinline__ int wave_units(const PlanShape& s, const PlanEntry& e, int tile) {
-  return tile < plan_tiles(s, e) ? plan_units(plan_span(s, e, tile)) : 0;
+__device__ __forceinline__ int64_t wave_units(const PlanShape& s, const PlanEntry& e, int tile) {
+  return tile < plan_tiles(s, e) ? plan_units(s, plan_span(s, e, tile)) : 0;
 }
 __device__ __forceinline__ int64_t wave_head_units(const PlanShape& s, const PlanEntry& e) {
   int64_t n = 0;
   const int tiles = plan_tiles(s, e);
-  for (int t = threadIdx.x & 63; t < tiles; t += 64) n += plan_units(plan_span(s, e, t));
+  for (int t = threadIdx.x & 63; t < tiles; t += 64) n += plan_units(s, plan_span(s, e, t));
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m, 64);
   return uniform(n);
 }
 __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
   const int lane = threadIdx.x & 63, tiles = plan_tiles(s, e);
-  const int64_t per_head = tiles == 1 ? plan_units(plan_span(s, e, 0)) : wave_head_units(s, e);
-  PlanPlace p = {entry, uniform((int)plan_div(rem, per_head)), 0, 0, 0};
+  const int64_t per_head = tiles == 1 ? plan_units(s, plan_span(s, e, 0)) : wave_head_units(s, e);
+  PlanPlace p = {entry, uniform((int)plan_div(rem, per_head)), 0, 0};
   rem -= p.head * per_head;
   start += p.head * per_head;
-  if (tiles == 1) {
-    p.at = (int)rem;
-    p.start = start;
-    return p;
-  }
+  p.start = start;
+  if (tiles == 1) return p;
   for (;; p.tile += 64) {
-    const int u = wave_units(s, e, p.tile + lane);
+    const int64_t u = wave_units(s, e, p.tile + lane);
     int64_t sum = u;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -138,31 +146,49 @@ __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEnt
     if (past == 0 && p.tile + 64 < tiles) {
       const int64_t all = uniform(__shfl(sum, 63, 64));
       rem -= all;
-      start += all;
+      p.start += all;
       continue;
     }
     const int at = past ? __builtin_ctzll(past) : 63;
-    const int64_t before = uniform(__shfl(sum - u, at, 64));
     p.tile += at;
-    p.at = (int)(rem - before);
-    p.start = start + before;
+    p.start += uniform(__shfl(sum - u, at, 64));
     return p;
   }
 }
 
 struct Run {
-  int64_t unit, end, per;
+  int w;  // the run's number
+  int64_t begin, end, per;
   PlanPlace place;
   Entry entry;
 };
 
-// The run of workgroup w of `groups`; false: it has none.
-__device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape& s, int w, int groups, int least,
-                                         Run& run) {
+// This workgroup's run; false: it has none.  Consecutive runs are on one XCD
+// (workgroups go round the eight), where they share K and V rows in its L2,
+// and the XCDs have equally many.
+constexpr int kXcds = 8;
+__device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape& s, int least, Run& run) {
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found_start;
   __shared__ int found[5];
   const int n = a.b.n;
+  // whether unit w per lies before `total`; sets the run's number and ends
+  auto cut = [&](int64_t total) {
+    run.per = plan_per(s, total, gridDim.x, least);
+    const int runs = (int)plan_div(total + run.per - 1, run.per), share = (runs + kXcds - 1) / kXcds;
+    run.w = (int)blockIdx.x % kXcds * share + (int)blockIdx.x / kXcds;
+    run.begin = run.w * run.per;
+    run.end = min(total, run.begin + run.per);
+    return (int)blockIdx.x / kXcds < share && run.begin < run.end;
+  };
+  if (n == 1) {  // nothing to add up: no barrier
+    run.entry = load_entry(a, 0);
+    if (!takes(a, run.entry.e.count)) return false;
+    const int64_t head = plan_tiles(s, run.entry.e) == 1 ? plan_units(s, plan_span(s, run.entry.e, 0)) : wave_head_units(s, run.entry.e);
+    if (!cut(s.heads * head)) return false;
+    run.place = wave_find(s, run.entry.e, 0, 0, run.begin);
+    return true;
+  }
   int2 rows, seq;
   auto units = [&](int b) -> int64_t {
     rows = seq = make_int2(0, 0);
@@ -192,10 +218,7 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
     total = all;
   }
   total = uniform(total);
-  run.per = plan_per(total, groups, least);
-  run.unit = w * run.per;
-  run.end = min(total, run.unit + run.per);
-  if (run.unit >= run.end) return false;
+  if (!cut(total)) return false;
   int64_t base = 0;
   for (int b0 = 0; b0 < n; b0 += kThreads) {
     int64_t chunk = 0;
@@ -206,7 +229,7 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
       mine = units(threadIdx.x);
       scan(mine, sums, chunk);
     }
-    if (before <= run.unit && run.unit < before + mine) {
+    if (before <= run.begin && run.begin < before + mine) {
       found[0] = b0 + threadIdx.x;
       found[1] = seq.x, found[2] = rows.x, found[3] = seq.y, found[4] = rows.y - rows.x;
       found_start = before;
@@ -217,15 +240,15 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
   const int b = uniform(found[0]);
   const int64_t start = uniform(found_start);
   run.entry = {uniform(found[1]), uniform(found[2]), {uniform(found[3]), uniform(found[4])}};
-  run.place = wave_find(s, run.entry.e, b, start, run.unit - start);
+  run.place = wave_find(s, run.entry.e, b, start, run.begin - start);
   return true;
 }
 
 // On to the next task.
-__device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShape& s, Run& run, int units) {
+__device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShape& s, Run& run) {
   PlanPlace& p = run.place;
-  p.at = 0;
-  p.start += units;
+  p.start += plan_units(s, plan_span(s, run.entry.e, p.tile));
+  if (p.start >= run.end) return;
   if (++p.tile < plan_tiles(s, run.entry.e)) return;
   p.tile = 0;
   if (++p.head < s.heads) return;
@@ -242,32 +265,34 @@ struct Task {
   Entry entry;
   const int32_t* table;  // the sequence's pages
   int64_t start;         // units before the task
-  int g, tile, r0, rows, pos0, units, take, kb0, kb1, seen;
+  int g, tile, r0, rows, pos0, blocks, kb0, kb1, seen;
+  bool cut;
 };
-__device__ __forceinline__ Task task_of(const PagedAttnArgs& a, const PlanShape& s, const Run& run) {
-  Task t;
-  const PlanSpan span = plan_span(s, run.entry.e, run.place.tile);
-  t.entry = run.entry;
-  t.table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
-  t.start = run.place.start;
-  t.g = run.place.head;
-  t.tile = run.place.tile;
-  t.r0 = run.place.tile * s.rows;
-  t.rows = min(s.rows, run.entry.e.count * a.group - t.r0);
-  t.pos0 = run.entry.e.length - run.entry.e.count;
-  t.units = plan_units(span);
-  t.take = (int)min((int64_t)(t.units - run.place.at), run.end - run.unit);
-  t.kb0 = span.lo + run.place.at;
-  t.kb1 = span.hi > span.lo ? t.kb0 + t.take : t.kb0;
-  t.seen = span.seen;
-  return t;
-}
 
-// Consecutive runs on one XCD (workgroups go round the eight XCDs), where they
-// share K and V rows in its L2.
-__device__ __forceinline__ int run_of_group() {
-  const int groups = gridDim.x;  // a multiple of 8
-  return (int)blockIdx.x % 8 * (groups / 8) + (int)blockIdx.x / 8;
+// The task at the run's place, or the next one of which the run has blocks;
+// false: there is none.
+__device__ __forceinline__ bool next_task(const PagedAttnArgs& a, const PlanShape& s, Run& run, Task& t) {
+  for (; run.place.start < run.end; plan_next(a, s, run)) {
+    const PlanSpan span = plan_span(s, run.entry.e, run.place.tile);
+    t.blocks = plan_blocks(span);
+    const PlanBlocks mine = plan_mine(s, run.place.start, t.blocks, run.begin, run.end);
+    if (mine.first >= mine.end) continue;
+    t.cut = mine.end - mine.first < t.blocks;
+    t.entry = run.entry;
+    t.table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
+    t.start = run.place.start;
+    t.g = run.place.head;
+    t.tile = run.place.tile;
+    t.r0 = run.place.tile * s.rows;
+    t.rows = min(s.rows, run.entry.e.count * a.group - t.r0);
+    t.pos0 = run.entry.e.length - run.entry.e.count;
+    t.kb0 = span.lo + mine.first;
+    t.kb1 = span.hi > span.lo ? span.lo + mine.end : t.kb0;
+    t.seen = span.seen;
+    plan_next(a, s, run);
+    return true;
+  }
+  return false;
 }
 
 // 2^(score - max): where all scores are -inf the maximum is no number to subtract.
@@ -294,9 +319,9 @@ __device__ __forceinline__ u32x2_t e4m3_bf16(uint32_t w) {
 // A task whose result is one of several parts: where it starts in the order of
 // units, and what is written when all parts are there.
 struct Pending {
-  int64_t start;
+  PlanParts parts;
   Entry entry;
-  int units, head, tile;
+  int head, tile;
 };
 
 // Once the workgroup's parts are stored: draws the tickets of its (at most
@@ -304,13 +329,13 @@ struct Pending {
 // have completed before the tickets are drawn (device-coherent stores, no L2
 // write-back as a fence would do).  The joining workgroup leaves the ticket at
 // zero.
-__device__ __forceinline__ int draw_tickets(const PagedAttnArgs& a, const Pending (&pend)[2], int n, int64_t per, int* last) {
+__device__ __forceinline__ int draw_tickets(const PagedAttnArgs& a, const Pending (&pend)[2], int n, int* last) {
   unsigned* const tickets = static_cast<unsigned*>(a.workspace);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if ((int)threadIdx.x < n) {
-    const Pending& p = threadIdx.x ? pend[1] : pend[0];
-    const PlanParts pp = plan_parts(p.start, p.units, per);
+    const PlanParts pp = {threadIdx.x ? pend[1].parts.first : pend[0].parts.first,
+                          threadIdx.x ? pend[1].parts.count : pend[0].parts.count};
     const bool is = __hip_atomic_fetch_add(tickets + pp.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                     (unsigned)(pp.count - 1);
     if (is) __hip_atomic_store(tickets + pp.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -341,7 +366,7 @@ __device__ __forceinline__ void rows_again(const PagedAttnArgs& a, const Entry& 
   const int32_t* const table = a.c.table + (int64_t)max(en.seq, 0) * a.c.width;
   const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e, vs = E4M3 ? a.c.v_scale[g] : 1.0f;
   for (int r = r0 + wave; r < r0 + rows; r += kWaves) {
-    const int tok = r / a.group, h = g * a.group + r - tok * a.group, p = en.e.length - en.e.count + tok;
+    const int tok = plan_div(r, a.by_group), h = g * a.group + r - tok * a.group, p = en.e.length - en.e.count + tok;
     const int64_t row = en.row0 + tok;
     const uint16_t* q = a.q + row * a.q_stride + h * D;
     float m = -INFINITY, l = 0.0f, o[kPer] = {};
@@ -417,10 +442,10 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   __shared__ int last[2], again[kWaves];
   constexpr int kJoin = D * NQ == 256 ? 8 : 16;  // parts at a time
   static_assert(4 * kJoin * N::kRows <= kWaves * N::kLds, "the weights fit the waves' LDS rows");
-  const PlanShape shape = {a.c.kv_heads, a.group, a.window, N::kRows, kWaves * kNarrowSlots};
-  const int w = run_of_group();
+  const PlanShape shape = {a.c.kv_heads, a.group, a.by_group, a.window, N::kRows, kWaves * kNarrowSlots, kBlockCost, kNarrowTaskCost};
   Run run;
-  if (!plan_run(a, shape, w, gridDim.x, 1, run)) return;
+  Task t;
+  if (!plan_run(a, shape, 1, run) || !next_task(a, shape, run, t)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, quad = lane >> 4;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
   char* const mylds = lds[wave];
@@ -429,7 +454,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   int pending = 0;
   // four dimensions of a finished row, and its lse
   auto finish = [&](const Entry& en, int g, int r, int d, const f32x4& x, float m, float l) {
-    const int tok = r / a.group, h = g * a.group + r - tok * a.group;
+    const int tok = plan_div(r, a.by_group), h = g * a.group + r - tok * a.group;
     const int64_t row = en.row0 + tok;
     const float f = l == 0.0f ? 0.0f : (E4M3 ? a.c.v_scale[g] : 1.0f) / l;
     u32x2_t y = {f32x2_to_bf16x2(x[0] * f, x[1] * f), f32x2_to_bf16x2(x[2] * f, x[3] * f)};
@@ -489,7 +514,6 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     find_pages(t, s0 + kWaves * kNarrowSlots);
   };
 
-  Task t = task_of(a, shape, run);
   begin(t);
   for (;;) {
     const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g;
@@ -501,7 +525,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     bf16x8 qf[NQ][N::kSteps];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int r = r0 + 16 * n + col, tok = r / a.group;
+      const int r = r0 + 16 * n + col, tok = plan_div(r, a.by_group);
       const bool ok = 16 * n + col < rows;
       pos[n] = ok ? pos0 + tok : -1;
       low[n] = a.window > 0 ? pos[n] - a.window : -1;
@@ -537,7 +561,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       // V into LDS (the reads of the tile before are done: their values have
       // been used).  Where not every row sees every slot, an infinity or NaN
       // among the values is noted for rows_again.
-      const int tok0 = r0 / a.group, tok1 = (r0 + rows - 1) / a.group;
+      const int tok0 = plan_div(r0, a.by_group), tok1 = plan_div(r0 + rows - 1, a.by_group);
       const bool whole = s0 + kNarrowSlots - 1 <= pos0 + tok0 && there == 3 &&
                          (a.window == 0 || s0 > pos0 + tok1 - a.window);
       bool bad = false;
@@ -643,13 +667,8 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
 
     // the next task's first loads are under way while this one ends
     const Task done = t;
-    run.unit += t.take;
-    const bool more_tasks = run.unit < run.end;
-    if (more_tasks) {
-      plan_next(a, shape, run, t.units);
-      t = task_of(a, shape, run);
-      begin(t);
-    }
+    const bool more_tasks = next_task(a, shape, run, t);
+    if (more_tasks) begin(t);
 
     // the waves' results meet: maxima and sums, then O through LDS 16 rows at a time
 #pragma unroll
@@ -664,8 +683,9 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       const int any = __any(poison);
       if (lane == 0) again[wave] = any;
     }
-    const bool cut = done.take < done.units;
-    const int slot = plan_slot(done.start, w, run.per) * (N::kPart * 4);
+    const bool cut = done.cut;
+    const PlanParts done_parts = cut ? plan_parts(shape, done.start, done.blocks, run.per) : PlanParts{0, 0};
+    const int slot = plan_slot(done_parts, run.w) * (N::kPart * 4);
     constexpr int kPer = D / 16;  // outputs of a thread: dimensions kPer (tid % 16) .. of row tid / 16
     const int orow = tid >> 4, od = kPer * (tid & 15);
     bool note = false;
@@ -712,14 +732,14 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     __syncthreads();  // the waves' V rows are free again
     if (!cut && note) rows_again<D, E4M3>(a, done.entry, g, r0, rows);
     if (cut) {
-      const Pending p = {done.start, done.entry, done.units, g, done.tile};
+      const Pending p = {done_parts, done.entry, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     }
     if (!more_tasks) break;
   }
 
-  const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
+  const int join = pending ? draw_tickets(a, pend, pending, last) : 0;
   // joins a task's parts, J at a time: all their loads go out at once, the
   // maxima and sums give each row's weights of the parts (kRowThreads threads
   // per row), and a thread adds up kItems words of four dimensions
@@ -727,14 +747,14 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   float (&weight)[kJoin][N::kRows] = *reinterpret_cast<float (*)[kJoin][N::kRows]>(&lds[0][0]);
   auto join_task = [&](const Pending& p, auto steps) {
     constexpr int J = decltype(steps)::value, kMine = (J + kRowThreads - 1) / kRowThreads;
-    const PlanParts pp = plan_parts(p.start, p.units, run.per);
+    const PlanParts pp = p.parts;
     const int r0 = p.tile * N::kRows, rows = min(N::kRows, p.entry.e.count * a.group - r0);
     const int row = tid / kRowThreads, sub = tid % kRowThreads;
     f32x4 x[kItems] = {};
     float m = -INFINITY, l = 0.0f;  // of row `row`, in each of its threads
     bool note = false;
     for (int k0 = 0; k0 < pp.count; k0 += J) {
-      auto part = [&](int k) { return plan_slot(p.start, pp.first + min(k0 + k, pp.count - 1), run.per) * (N::kPart * 4); };
+      auto part = [&](int k) { return plan_slot(pp, pp.first + min(k0 + k, pp.count - 1)) * (N::kPart * 4); };
       float pm[kMine], pl[kMine];
       u32x4 y[kItems][J];
 #pragma unroll
@@ -801,9 +821,9 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   };
   for (int j = 0; j < 2; ++j) {
     if (!((join >> j) & 1)) continue;
-    const Pending& p = j ? pend[1] : pend[0];
+    const Pending p = j ? pend[1] : pend[0];
     __syncthreads();  // (wm and wl of another task have been read)
-    if (plan_parts(p.start, p.units, run.per).count <= 4)
+    if (p.parts.count <= 4)
       join_task(p, std::integral_constant<int, 4>());
     else
       join_task(p, std::integral_constant<int, kJoin>());
@@ -864,10 +884,10 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
   __shared__ __attribute__((aligned(16))) int note_lds[2][kWaves];
   __shared__ int last[2], again[kWaves];
   constexpr int kQuads = D / 8;  // 16-byte words of a part's O per lane and QB
-  const PlanShape shape = {a.c.kv_heads, a.group, a.window, W::kRows, kWideSlots};
-  const int w = run_of_group();
+  const PlanShape shape = {a.c.kv_heads, a.group, a.by_group, a.window, W::kRows, kWideSlots, kBlockCost, kWideTaskCost};
   Run run;
-  if (!plan_run(a, shape, w, gridDim.x, 4, run)) return;
+  Task t;
+  if (!plan_run(a, shape, 4, run) || !next_task(a, shape, run, t)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
   const __amdgpu_buffer_rsrc_t parts = parts_of(a);
@@ -880,7 +900,7 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     for (int b = 0; b < QB; ++b) {
       const int at = 32 * (QB * wave + b) + col;
       if (at >= rows) continue;
-      const int tok = (r0 + at) / a.group, h = g * a.group + (r0 + at) - tok * a.group;
+      const int tok = plan_div(r0 + at, a.by_group), h = g * a.group + (r0 + at) - tok * a.group;
       const int64_t row = en.row0 + tok;
       const float l = ls[b], f = l == 0.0f ? 0.0f : vs / l;
       uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
@@ -926,21 +946,20 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     find_page(t, (t.kb0 + 1) * kWideSlots);
   };
 
-  Task t = task_of(a, shape, run);
   begin(t);
   for (;;) {
     const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g, kb0 = t.kb0, kb1 = t.kb1;
     const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
     // the wave's rows [w0, w1) of the tile, and the positions they span
     const int w0 = wave * 32 * QB, w1 = min(rows, w0 + 32 * QB);
-    const int wave_lo = pos0 + (r0 + w0) / a.group, wave_hi = w1 > w0 ? pos0 + (r0 + w1 - 1) / a.group : -1;
-    const int tile_lo = pos0 + r0 / a.group, tile_hi = pos0 + (r0 + rows - 1) / a.group;
+    const int wave_lo = pos0 + plan_div(r0 + w0, a.by_group), wave_hi = w1 > w0 ? pos0 + plan_div(r0 + w1 - 1, a.by_group) : -1;
+    const int tile_lo = pos0 + plan_div(r0, a.by_group), tile_hi = pos0 + plan_div(r0 + rows - 1, a.by_group);
 
     int pos[QB], low[QB];
     bf16x8 qf[QB][kSteps];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-      const int at = w0 + 32 * b + col, r = r0 + at, tok = r / a.group;
+      const int at = w0 + 32 * b + col, r = r0 + at, tok = plan_div(r, a.by_group);
       const bool ok = at < rows;
       pos[b] = ok ? pos0 + tok : -1;
       low[b] = a.window > 0 ? pos[b] - a.window : -1;
@@ -1128,14 +1147,10 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
 
     // the next task's first loads are under way while this one ends
     const Task done = t;
-    run.unit += t.take;
-    const bool more_tasks = run.unit < run.end;
-    if (more_tasks) {
-      plan_next(a, shape, run, t.units);
-      t = task_of(a, shape, run);
-      begin(t);
-    }
-    const bool cut = done.take < done.units;
+    const bool more_tasks = next_task(a, shape, run, t);
+    if (more_tasks) begin(t);
+    const bool cut = done.cut;
+    const PlanParts done_parts = cut ? plan_parts(shape, done.start, done.blocks, run.per) : PlanParts{0, 0};
 #pragma unroll
     for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
     if (lane == 0) again[wave] = poison;
@@ -1143,7 +1158,7 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     const bool note = again[0] | again[1] | again[2] | again[3];
     if (cut) {
       // parts lie lane by lane: word i of thread t at 16 (i threads + t) bytes
-      const int slot = plan_slot(done.start, w, run.per) * (W::kPart * 4);
+      const int slot = plan_slot(done_parts, run.w) * (W::kPart * 4);
       if (wave_hi >= 0) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
@@ -1159,7 +1174,7 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
                                                 slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
         }
       }
-      const Pending p = {done.start, done.entry, done.units, g, done.tile};
+      const Pending p = {done_parts, done.entry, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     } else if (note) {
@@ -1171,14 +1186,14 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     if (!more_tasks) break;
   }
 
-  const int join = pending ? draw_tickets(a, pend, pending, run.per, last) : 0;
+  const int join = pending ? draw_tickets(a, pend, pending, last) : 0;
   for (int j = 0; j < 2; ++j) {
     if (!((join >> j) & 1)) continue;
-    const Pending& p = j ? pend[1] : pend[0];
-    const PlanParts pp = plan_parts(p.start, p.units, run.per);
+    const Pending p = j ? pend[1] : pend[0];
+    const PlanParts pp = p.parts;
     const int r0 = p.tile * W::kRows, rows = min(W::kRows, p.entry.e.count * a.group - r0);
     // (a wave whose rows stand at negative positions has no part)
-    const bool has = p.entry.e.length - p.entry.e.count + (r0 + min(rows, 32 * QB * (wave + 1)) - 1) / a.group >= 0 &&
+    const bool has = p.entry.e.length - p.entry.e.count + plan_div(r0 + min(rows, 32 * QB * (wave + 1)) - 1, a.by_group) >= 0 &&
                      rows > 32 * QB * wave;
     float m[QB], l[QB];
     f32x16 o[QB][kDims];
@@ -1193,7 +1208,7 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
         for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
       if (!has) continue;
       for (int k = 0; k < pp.count; ++k) {
-        const int slot = plan_slot(p.start, pp.first + k, run.per) * (W::kPart * 4);
+        const int slot = plan_slot(pp, pp.first + k) * (W::kPart * 4);
         const u32x2_t ml =
             __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
         u32x4 y[kQuads];
@@ -1248,6 +1263,7 @@ void narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
 template <int D, bool E4M3>
 void launch(PagedAttnArgs a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_new * a.group;
+  a.by_group = plan_divisor(a.group);
   a.rows_min = 1;
   a.rows_max = INT32_MAX;
   if (rows <= 64) return narrow<D, E4M3>(a, rows, stream);

@@ -3,10 +3,11 @@
 //
 // A task is one tile of an entry's rows (row r: token r / group, query head
 // r % group of the kv head) over the blocks of slots that one of them sees.
-// Tasks stand in the order entry, kv head, tile; a block is a unit of work, a
-// task that sees nothing one unit too (its rows are still written).  Workgroup
-// w takes the units [w per, (w + 1) per): whole tasks, and at its ends parts of
-// tasks, whose results meet in the workspace.
+// Tasks stand in the order entry, kv head, tile.  A task costs task_cost units
+// of its own and block_cost for each of its blocks; one that sees nothing has
+// an empty block all the same (its rows are still written).  Workgroup w takes
+// the blocks that begin in the units [w per, (w + 1) per): whole tasks, and at
+// its ends parts of tasks, whose results meet in the workspace.
 #pragma once
 
 #include <stdint.h>
@@ -19,12 +20,28 @@
 
 namespace hk {
 
+// x / d for 0 <= x < 2^31 as a product: x * ceil(2^(31 + L) / d) >> (31 + L)
+// with 2^L >= d (Granlund and Montgomery, Division by invariant integers using
+// multiplication).  A division by a variable is forty instructions.
+struct PlanDivisor {
+  uint32_t mul;
+  int shift;
+};
+HK_PLAN PlanDivisor plan_divisor(int d) {
+  int l = 0;
+  while ((1 << l) < d) ++l;
+  return {(uint32_t)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+}
+HK_PLAN int plan_div(int x, const PlanDivisor& d) { return (int)(((uint64_t)(uint32_t)x * d.mul) >> d.shift); }
+
 struct PlanShape {
   int heads;   // kv heads
   int group;   // query heads per kv head
+  PlanDivisor by_group;
   int window;  // 0: none
   int rows;    // of a tile
   int slots;   // of a block
+  int block_cost, task_cost;  // units
 };
 
 struct PlanEntry {
@@ -40,19 +57,22 @@ HK_PLAN int plan_tiles(const PlanShape& s, const PlanEntry& e) { return (e.count
 
 HK_PLAN PlanSpan plan_span(const PlanShape& s, const PlanEntry& e, int tile) {
   const int r0 = tile * s.rows, end = r0 + s.rows < e.count * s.group ? r0 + s.rows : e.count * s.group;
-  const int p0 = e.length - e.count + r0 / s.group, p1 = e.length - e.count + (end - 1) / s.group;
+  const int p0 = e.length - e.count + plan_div(r0, s.by_group), p1 = e.length - e.count + plan_div(end - 1, s.by_group);
   const int low = s.window > 0 && p0 >= s.window ? p0 - s.window + 1 : 0;
   if (p1 < low) return {0, 0, 0};
   return {low / s.slots, p1 / s.slots + 1, p1 + 1};
 }
 
-HK_PLAN int plan_units(const PlanSpan& s) { return s.hi > s.lo ? s.hi - s.lo : 1; }
+HK_PLAN int plan_blocks(const PlanSpan& s) { return s.hi > s.lo ? s.hi - s.lo : 1; }
+HK_PLAN int64_t plan_units(const PlanShape& s, const PlanSpan& span) {
+  return s.task_cost + (int64_t)s.block_cost * plan_blocks(span);
+}
 
 // Units of one kv head of an entry.
 HK_PLAN int64_t plan_head_units(const PlanShape& s, const PlanEntry& e) {
   int64_t n = 0;
   const int tiles = plan_tiles(s, e);
-  for (int t = 0; t < tiles; ++t) n += plan_units(plan_span(s, e, t));
+  for (int t = 0; t < tiles; ++t) n += plan_units(s, plan_span(s, e, t));
   return n;
 }
 
@@ -62,47 +82,60 @@ HK_PLAN int64_t plan_div(int64_t a, int64_t b) {
   return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-HK_PLAN int64_t plan_per(int64_t total, int groups, int least) {
-  const int64_t per = plan_div(total + groups - 1, groups);
-  return per > least ? per : least;
+// Units per workgroup; at least a block, so that every workgroup between a
+// task's first and last has a block of it.
+HK_PLAN int64_t plan_per(const PlanShape& s, int64_t total, int groups, int least) {
+  const int64_t per = plan_div(total + groups - 1, groups), most = (int64_t)least * s.block_cost;
+  return per > most ? per : most;
 }
 
-// A place in the order of tasks: `at` units of the task lie before it, `start`
-// units before the task.
+// A task's place in the order: `start` units lie before it.
 struct PlanPlace {
   int entry, head, tile;
-  int at;
   int64_t start;
 };
 
-// The place `rem` units into entry `entry`, which starts at unit `start`.
+// The task that unit `rem` of entry `entry` belongs to; the entry starts at
+// unit `start`.
 HK_PLAN PlanPlace plan_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
   const int64_t per_head = plan_head_units(s, e);
-  PlanPlace p = {entry, (int)plan_div(rem, per_head), 0, 0, 0};
+  PlanPlace p = {entry, (int)plan_div(rem, per_head), 0, 0};
   rem -= p.head * per_head;
-  start += p.head * per_head;
+  p.start = start + p.head * per_head;
   for (;;) {
-    const int u = plan_units(plan_span(s, e, p.tile));
-    if (rem < u) break;
+    const int64_t u = plan_units(s, plan_span(s, e, p.tile));
+    if (rem < u) return p;
     rem -= u;
-    start += u;
+    p.start += u;
     ++p.tile;
   }
-  p.at = (int)rem;
-  p.start = start;
-  return p;
 }
 
-// Parts of a task of `units` units from `start`: the workgroups that have
-// some, and the place of workgroup w's part among the partial results (two
-// per workgroup: the task it goes on with, and the task it begins).
+// The blocks [first, end) of a task that begin in the units [u0, u1).
+struct PlanBlocks {
+  int first, end;
+};
+HK_PLAN int plan_block_at(const PlanShape& s, int64_t start, int blocks, int64_t u) {
+  const int64_t past = u - start - s.task_cost;
+  if (past <= 0) return 0;
+  const int64_t k = plan_div(past + s.block_cost - 1, s.block_cost);
+  return k < blocks ? (int)k : blocks;
+}
+HK_PLAN PlanBlocks plan_mine(const PlanShape& s, int64_t start, int blocks, int64_t u0, int64_t u1) {
+  return {plan_block_at(s, start, blocks, u0), plan_block_at(s, start, blocks, u1)};
+}
+
+// The workgroups that have blocks of a task, and the place of workgroup w's
+// part among the partial results.  Each workgroup has two: for the task that it
+// goes on with, and for the one that it begins (whose first block is its own).
 struct PlanParts {
   int first, count;
 };
-HK_PLAN PlanParts plan_parts(int64_t start, int units, int64_t per) {
-  const int first = (int)plan_div(start, per), last = (int)plan_div(start + units - 1, per);
+HK_PLAN PlanParts plan_parts(const PlanShape& s, int64_t start, int blocks, int64_t per) {
+  start += s.task_cost;
+  const int first = (int)plan_div(start, per), last = (int)plan_div(start + (int64_t)s.block_cost * (blocks - 1), per);
   return {first, last - first + 1};
 }
-HK_PLAN int plan_slot(int64_t start, int w, int64_t per) { return 2 * w + (start >= w * per ? 1 : 0); }
+HK_PLAN int plan_slot(const PlanParts& p, int w) { return 2 * w + (w == p.first ? 1 : 0); }
 
 }  // namespace hk

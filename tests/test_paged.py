@@ -234,44 +234,50 @@ PLAN = """
 using namespace hk;
 #define CHECK(x) if (!(x)) { std::printf("%s, seed %d\\n", #x, seed); return 1; }
 int main() {
+  for (int d = 1, seed = 0; d <= 4096; ++d)
+    for (int64_t q = 0; q <= INT32_MAX / d; q = q < 20 || q * d > INT32_MAX - 20 * d ? q + 1 : q + INT32_MAX / d / 7)
+      for (int64_t x : {q * d, q * d + d - 1})
+        if (x <= INT32_MAX) CHECK(plan_div((int)x, plan_divisor(d)) == x / d);
   for (int seed = 0; seed < 400; ++seed) {
     std::mt19937 rng(seed);
     auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
     const int rows[] = {16, 32, 64, 256}, slots[] = {64, 128};
-    PlanShape s{pick(1, 4), pick(1, 9), pick(0, 2) ? 0 : pick(1, 300), rows[pick(0, 3)], slots[pick(0, 1)]};
+    const int group = pick(1, 9);
+    PlanShape s{pick(1, 4), group, plan_divisor(group), pick(0, 2) ? 0 : pick(1, 300), rows[pick(0, 3)], slots[pick(0, 1)], pick(1, 3),
+                pick(0, 5)};
     std::vector<PlanEntry> e(pick(1, 12));
     for (auto& x : e) x = {pick(0, 3) ? pick(0, 2000) : 0, pick(0, 3) ? pick(0, 3) : pick(0, 700)};
     int64_t total = 0;
     std::vector<int64_t> start;
     for (auto& x : e) start.push_back(total), total += s.heads * plan_head_units(s, x);
     const int groups = pick(1, 40);
-    const int64_t per = plan_per(total, groups, pick(1, 4));
-    std::map<std::tuple<int, int, int>, std::vector<int>> got;  // task: units
+    const int64_t per = plan_per(s, total, groups, pick(1, 4));
+    CHECK(groups * per >= total);
+    std::map<std::tuple<int, int, int>, std::vector<int>> got;  // task: blocks
     std::map<std::tuple<int, int, int>, int> arrived, asked, ticket;
     std::set<int> partials;
     for (int w = 0; w < groups; ++w) {
-      int64_t u = w * per;
-      const int64_t end = std::min(total, u + per);
-      if (u >= end) continue;
+      const int64_t begin = w * per, end = std::min(total, begin + per);
+      if (begin >= end) continue;
       size_t i = 0;
-      while (i + 1 < e.size() && start[i + 1] <= u) ++i;
-      PlanPlace p = plan_find(s, e[i], (int)i, start[i], u - start[i]);
-      while (u < end) {
+      while (i + 1 < e.size() && start[i + 1] <= begin) ++i;
+      PlanPlace p = plan_find(s, e[i], (int)i, start[i], begin - start[i]);
+      CHECK(p.start <= begin);
+      while (p.entry < (int)e.size() && p.start < end) {
         const PlanSpan span = plan_span(s, e[p.entry], p.tile);
-        const int units = plan_units(span), take = (int)std::min<int64_t>(units - p.at, end - u);
+        const int blocks = plan_blocks(span);
+        const PlanBlocks mine = plan_mine(s, p.start, blocks, begin, end);
+        const PlanParts parts = plan_parts(s, p.start, blocks, per);
         const auto task = std::make_tuple(p.entry, p.head, p.tile);
-        CHECK(p.start + p.at == u && take > 0);
-        for (int k = 0; k < take; ++k) got[task].push_back(p.at + k);
-        if (take < units) {
-          const PlanParts parts = plan_parts(p.start, units, per);
-          const int slot = plan_slot(p.start, w, per);
-          CHECK(w >= parts.first && w < parts.first + parts.count && parts.count > 1);
-          CHECK(partials.insert(slot).second && slot < 2 * groups);
+        CHECK((mine.first < mine.end) == (w >= parts.first && w < parts.first + parts.count));
+        for (int k = mine.first; k < mine.end; ++k) got[task].push_back(k);
+        if (mine.first < mine.end && mine.end - mine.first < blocks) {
+          const int slot = plan_slot(parts, w);
+          CHECK(parts.count > 1 && partials.insert(slot).second && slot < 2 * groups);
           CHECK(!ticket.count(task) || ticket[task] == parts.first);
           ticket[task] = parts.first, asked[task] = parts.count, ++arrived[task];
         }
-        u += take;
-        p.at = 0, p.start += units;
+        p.start += plan_units(s, span);
         if (++p.tile >= plan_tiles(s, e[p.entry])) {
           p.tile = 0;
           if (++p.head >= s.heads) {
@@ -283,16 +289,16 @@ int main() {
     }
     std::set<int> tickets;
     for (auto& t : ticket) CHECK(tickets.insert(t.second).second && asked[t.first] == arrived[t.first]);
-    // every task once, its units in order; every slot that a row sees inside a block of its tile
+    // every task once, its blocks in order; every slot that a row sees inside a block of its tile
     size_t tasks = 0;
     for (size_t i = 0; i < e.size(); ++i)
       for (int t = 0; t < plan_tiles(s, e[i]); ++t) {
         const PlanSpan span = plan_span(s, e[i], t);
         tasks += s.heads;
         for (int h = 0; h < s.heads; ++h) {
-          const auto& units = got[std::make_tuple((int)i, h, t)];
-          CHECK((int)units.size() == plan_units(span));
-          for (size_t k = 0; k < units.size(); ++k) CHECK(units[k] == (int)k);
+          const auto& blocks = got[std::make_tuple((int)i, h, t)];
+          CHECK((int)blocks.size() == plan_blocks(span));
+          for (size_t k = 0; k < blocks.size(); ++k) CHECK(blocks[k] == (int)k);
         }
         for (int r = t * s.rows; r < std::min((t + 1) * s.rows, e[i].count * s.group); ++r) {
           const int p = e[i].length - e[i].count + r / s.group, low = s.window ? std::max(0, p - s.window + 1) : 0;
