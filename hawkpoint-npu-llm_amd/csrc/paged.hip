@@ -251,7 +251,7 @@ struct ForkArgs {
   int32_t* status;
   int n, pages, seqs, width, page_shift;
   // workspace: the entries as read, and what they get
-  int* entry;    // [7][n]: child, parent, keep, total pages, first new page, wanted page, old pages
+  int* entry;    // [7][n] (LDS false)
   int* owner;    // [seqs] first entry of a child
   int* claim;    // [pages] first entry that wants a page
   int* fresh;    // [pages] free pages in order
@@ -260,22 +260,30 @@ struct ForkArgs {
   int* count;    // moves
 };
 
+// Up to kForkLds entries are kept in LDS, more in the workspace.  What it takes
+// is round trips to memory, one after the other (about a microsecond each, ten
+// of them): the rows of all entries are gone through together, a thread per
+// (entry, column), where a wave per entry took 68 us for 192 entries.
+constexpr int kForkLds = 1024;
+template <bool LDS>
 __global__ __launch_bounds__(kBook) void paged_fork_kernel(ForkArgs a) {
   __shared__ int sums[kBookWaves];
-  __shared__ int bad;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, shift = a.page_shift;
-  int* const child = a.entry;
-  int* const parent = child + n;
-  int* const keep = parent + n;
-  int* const total = keep + n;
-  int* const start = total + n;
-  int* const want = start + n;
-  int* const held = want + n;
+  __shared__ int bad, moved, longest;
+  __shared__ int entry_lds[LDS ? 7 * kForkLds : 1];
+  const int tid = threadIdx.x, n = a.n, shift = a.page_shift, stride = LDS ? kForkLds : n;
+  int* const child = LDS ? entry_lds : a.entry;
+  int* const parent = child + stride;
+  int* const keep = parent + stride;
+  int* const total = keep + stride;  // pages
+  int* const start = total + stride; // first of its new pages
+  int* const want = start + stride;  // the partly filled page; ~page - 1: taken over; -1: none
+  int* const held = want + stride;   // pages before the call
   const int slots = a.width << shift, mask = (1 << shift) - 1;
   auto length = [&](int s) { return min(max(a.length[s], 0), slots); };
   if (tid == 0) {
     bad = n;
-    *a.count = 0;
+    moved = 0;
+    longest = 1;
   }
   for (int i = tid; i < n; i += kBook) {
     const int c = a.child ? a.child[i] : i;
@@ -292,11 +300,13 @@ __global__ __launch_bounds__(kBook) void paged_fork_kernel(ForkArgs a) {
     int w = -1;
     if (ok) {
       __hip_atomic_fetch_min(a.owner + c, i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int t = (int)((k + g + mask) >> shift), h = (length(c) + mask) >> shift;
       child[i] = c;
       parent[i] = has ? q : c;
       keep[i] = (int)k;
-      total[i] = (int)((k + g + mask) >> shift);
-      held[i] = (length(c) + mask) >> shift;
+      total[i] = t;
+      held[i] = h;
+      atomicMax(&longest, max(t, h) - (!has || q == c ? (int)(k >> shift) : 0));
       if (k & mask) {
         w = a.table[(int64_t)q * a.width + (k >> shift)];
         ok = (unsigned)w < (unsigned)a.pages;
@@ -314,26 +324,38 @@ __global__ __launch_bounds__(kBook) void paged_fork_kernel(ForkArgs a) {
   if (mine < n) atomicMin(&bad, mine);
   __syncthreads();
   if (bad < n) {
-    if (tid == 0) a.status[0] = HK_PAGED_BAD_ENTRY, a.status[1] = bad;
+    if (tid == 0) {
+      *a.count = 0;
+      a.status[0] = HK_PAGED_BAD_ENTRY, a.status[1] = bad;
+    }
     return;
   }
-  // the counts without what the children held and with what they share; an
-  // entry that goes on from itself keeps its full pages without either.
-  // Then (by < 0) the same taken back.
-  auto share = [&](int by) {
-    for (int i = wave; i < n; i += kBookWaves) {
-      const bool self = child[i] == parent[i];
-      const int full = keep[i] >> shift, old = held[i];
-      const int32_t* had = a.table + (int64_t)child[i] * a.width;
-      for (int j = (self ? full : 0) + lane; j < old; j += 64)
-        if ((unsigned)had[j] < (unsigned)a.pages) bump(a.refs + had[j], -by);
-      if (self) continue;
-      const int32_t* src = a.table + (int64_t)parent[i] * a.width;
-      for (int j = lane; j < full; j += 64) {
-        if ((unsigned)src[j] < (unsigned)a.pages) bump(a.refs + src[j], by);
-        a.rows[(int64_t)i * a.width + j] = src[j];
-      }
+  // f(entry, column) for every entry and the columns that the call concerns: an
+  // entry that goes on from itself keeps its full pages without a look
+  int columns = 0;
+  while ((1 << columns) < longest) ++columns;
+  auto cells = [&](auto f) {
+    const int64_t all = (int64_t)n << columns;
+    for (int64_t x = tid; x < all; x += kBook) {
+      const int i = (int)(x >> columns), j = (int)(x & ((1 << columns) - 1)) + (child[i] == parent[i] ? keep[i] >> shift : 0);
+      f(i, j);
     }
+  };
+  // the counts without what the children held and with what they share (by 1);
+  // the same taken back (by -1)
+  auto share = [&](int by) {
+    cells([&](int i, int j) {
+      const int full = keep[i] >> shift;
+      if (j < held[i]) {
+        const int p = a.table[(int64_t)child[i] * a.width + j];
+        if ((unsigned)p < (unsigned)a.pages) bump(a.refs + p, -by);
+      }
+      if (j < full) {  // (never of the sequence itself)
+        const int p = a.table[(int64_t)parent[i] * a.width + j];
+        if ((unsigned)p < (unsigned)a.pages) bump(a.refs + p, by);
+        a.rows[(int64_t)i * a.width + j] = p;
+      }
+    });
   };
   share(1);
   for (int i = tid; i < n; i += kBook)
@@ -346,13 +368,16 @@ __global__ __launch_bounds__(kBook) void paged_fork_kernel(ForkArgs a) {
   for (int i = i0; i < i1; ++i) {
     bool taken = false;
     if (want[i] >= 0) taken = peek(a.refs + want[i]) <= 0 && peek(a.claim + want[i]) == i;
-    if (taken) want[i] = ~want[i] - 1;  // below -1: the page itself
+    if (taken) want[i] = ~want[i] - 1;
     need += total[i] - (keep[i] >> shift) - (taken ? 1 : 0);
   }
   int all, before;
   const int offset = book_scan(need, sums, all);  // (its barriers come before the counts change)
-  for (int i = i0; i < i1; ++i)
+  for (int i = i0, at = offset; i < i1; ++i) {
     if (want[i] < -1) poke(a.refs + ~(want[i] + 1), 1);
+    start[i] = at;
+    at += total[i] - (keep[i] >> shift) - (want[i] < -1 ? 1 : 0);
+  }
   book_sync();
   const int free_pages = book_count<true>(a.refs, 0, a.pages, sums, before);
   if (free_pages < all) {
@@ -360,36 +385,41 @@ __global__ __launch_bounds__(kBook) void paged_fork_kernel(ForkArgs a) {
       if (want[i] < -1) poke(a.refs + ~(want[i] + 1), 0);
     book_sync();
     share(-1);
-    if (tid == 0) a.status[0] = HK_PAGED_FULL, a.status[1] = all - free_pages;
+    if (tid == 0) {
+      *a.count = 0;
+      a.status[0] = HK_PAGED_FULL, a.status[1] = all - free_pages;
+    }
     return;
   }
   book_list<true>(a.refs, 0, a.pages, before, all, [&](int rank, int page) { a.fresh[rank] = page; });
-  for (int i = i0, at = offset; i < i1; ++i) {
-    start[i] = at;
-    at += total[i] - (keep[i] >> shift) - (want[i] < -1 ? 1 : 0);
-  }
   book_sync();
   for (int r = tid; r < all; r += kBook) poke(a.refs + a.fresh[r], 1);
-  // the rows, lengths and copies
-  for (int i = wave; i < n; i += kBookWaves) {
-    const int full = keep[i] >> shift;
-    const bool taken = want[i] < -1;
-    int32_t* row = a.table + (int64_t)child[i] * a.width;
-    if (child[i] != parent[i])
-      for (int j = lane; j < full; j += 64) row[j] = a.rows[(int64_t)i * a.width + j];
-    if (taken && lane == 0) row[full] = ~(want[i] + 1);
-    for (int j = full + taken + lane; j < total[i]; j += 64) row[j] = a.fresh[start[i] + j - full - taken];
-    for (int j = total[i] + lane; j < held[i]; j += 64) row[j] = -1;
-    if (lane == 0 && want[i] >= 0) {
-      const int at = atomicAdd(a.count, 1);
-      a.moves[at] = Move{want[i], a.fresh[start[i]], keep[i] & mask};
-    }
-  }
+  // the rows, the copies and the lengths
+  cells([&](int i, int j) {
+    const int full = keep[i] >> shift, taken = want[i] < -1;
+    int p;
+    if (j < full)
+      p = a.rows[(int64_t)i * a.width + j];
+    else if (j < full + taken)
+      p = ~(want[i] + 1);
+    else if (j < total[i])
+      p = a.fresh[start[i] + j - full - taken];
+    else if (j < held[i])
+      p = -1;
+    else
+      return;
+    a.table[(int64_t)child[i] * a.width + j] = p;
+  });
+  for (int i = tid; i < n; i += kBook)
+    if (want[i] >= 0) a.moves[atomicAdd(&moved, 1)] = Move{want[i], a.fresh[start[i]], keep[i] & mask};
   book_sync();
   for (int i = tid; i < n; i += kBook) start[i] = keep[i] + (a.grow ? a.grow[i] : 0);
   book_sync();  // (grow may be the lengths)
   for (int i = tid; i < n; i += kBook) a.length[child[i]] = start[i];
-  if (tid == 0) a.status[0] = HK_PAGED_DONE, a.status[1] = 0;
+  if (tid == 0) {
+    *a.count = moved;
+    a.status[0] = HK_PAGED_DONE, a.status[1] = 0;
+  }
 }
 
 // ---- compaction ----
@@ -662,7 +692,10 @@ int hk_paged_fork(const hk_paged_cache* cache, const int32_t* child, const int32
   a.rows = a.fresh + a.pages;
   a.moves = reinterpret_cast<Move*>(a.rows + (int64_t)n * a.width);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(paged_fork_kernel, dim3(1), dim3(kBook), 0, st, a);
+  if (n <= kForkLds)
+    hipLaunchKernelGGL(paged_fork_kernel<true>, dim3(1), dim3(kBook), 0, st, a);
+  else
+    hipLaunchKernelGGL(paged_fork_kernel<false>, dim3(1), dim3(kBook), 0, st, a);
   HK_TRY(launched("paged fork launch"));
   hipLaunchKernelGGL(paged_move_kernel, dim3(kMoveGroups), dim3(256), 0, st, moves_of(cache, a.moves, a.count, false));
   return launched("paged fork copy launch");
