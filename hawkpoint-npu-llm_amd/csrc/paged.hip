@@ -1,6 +1,5 @@
 // The paged KV cache's entry points (include/hk_paged.h) and the kernels of
 // its append, fork and compaction.  The attention is in paged_attention.hip.
-#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -139,22 +138,52 @@ struct MoveArgs {
   int64_t layer_bytes, page_bytes;
   int layers, kv_heads, page_shift, row_bytes;
   int whole;  // every move is of whole pages, whose heads are one run
+  // compaction: the tables' cells, and the new numbers of the pages from `live` on
+  const int32_t* table;
+  int32_t* table_out;
+  const int32_t* live;
+  const int* place;
+  int64_t cells;
+  int pages;
 };
 
-// Runs (move, layer, keys or values, head) go round the workgroups.
+// Pieces of 16 KiB of the runs (move, layer, keys or values, head) go round the
+// workgroups; before that the tables get the pages' new numbers, where there
+// are any.  What bounds it is memory: 475 pages of 2 MB moved in 406 us (4.9
+// TB/s read and written, a large copy reaches 4.7), a prompt's page copied to 8
+// answers at 5.9.  The stores stream, as nobody reads the copies soon (134 us
+// for 192 answers against 156); the loads do not, as a page may be the source of
+// several copies (streaming loads too: 172; without several copies 402 and 406).
+constexpr int kPieceLoads = 4;
+constexpr int kPieceBytes = 256 * 16 * kPieceLoads;
 __global__ __launch_bounds__(256) void paged_move_kernel(MoveArgs a) {
   const int heads = a.whole ? 1 : a.kv_heads, per_move = a.layers * 2 * heads;
-  const int64_t runs = (int64_t)*a.count * per_move;
-  const int64_t head_bytes = (int64_t)a.row_bytes << a.page_shift;
-  for (int64_t i = blockIdx.x; i < runs; i += gridDim.x) {
-    const Move m = a.moves[i / per_move];
-    const int r = (int)(i % per_move), h = r % heads, kv = r / heads % 2, layer = r / heads / 2;
+  const int64_t head_bytes = (int64_t)a.row_bytes << a.page_shift, most = a.whole ? head_bytes * a.kv_heads : head_bytes;
+  const int pieces = (int)((most + kPieceBytes - 1) / kPieceBytes);
+  if (a.cells) {
+    const int first = *a.live;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.cells; i += (int64_t)gridDim.x * 256) {
+      const int p = a.table[i];
+      a.table_out[i] = p >= first && p < a.pages ? a.place[p] : p;
+    }
+  }
+  const int64_t all = (int64_t)*a.count * per_move * pieces;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const int64_t run = i / pieces;
+    const Move m = a.moves[run / per_move];
+    const int r = (int)(run % per_move), h = r % heads, kv = r / heads % 2, layer = r / heads / 2;
     char* pool = (kv ? a.v : a.k) + layer * a.layer_bytes + h * head_bytes;
-    const char* src = pool + m.from * a.page_bytes;
-    char* dst = pool + m.to * a.page_bytes;
-    const int64_t bytes = a.whole ? head_bytes * a.kv_heads : (int64_t)m.slots * a.row_bytes;
-    for (int64_t b = threadIdx.x * 16; b < bytes; b += 256 * 16)
-      stg(reinterpret_cast<u32x4*>(dst + b), load16(src + b));
+    const int64_t at = (i - run * pieces) * kPieceBytes + threadIdx.x * 16;
+    const int64_t bytes = (a.whole ? most : (int64_t)m.slots * a.row_bytes) - at;
+    const char* src = pool + m.from * a.page_bytes + at;
+    char* dst = pool + m.to * a.page_bytes + at;
+    u32x4 x[kPieceLoads];
+#pragma unroll
+    for (int k = 0; k < kPieceLoads; ++k)
+      if (k * 4096 < bytes) x[k] = load16(src + k * 4096);
+#pragma unroll
+    for (int k = 0; k < kPieceLoads; ++k)
+      if (k * 4096 < bytes) __builtin_nontemporal_store(x[k], (__attribute__((address_space(1))) u32x4*)(dst + k * 4096));
   }
 }
 
@@ -459,16 +488,6 @@ __global__ __launch_bounds__(kBook) void paged_compact_kernel(CompactArgs a) {
   if (tid == 0) *a.live = live, *a.count = movers;
 }
 
-// The tables with the pages' new numbers.
-__global__ __launch_bounds__(256) void paged_rename_kernel(const int32_t* table, int32_t* out, int64_t n,
-                                                           const int32_t* live, const int* place, int pages) {
-  const int first = *live;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int p = table[i];
-    out[i] = p >= first && p < pages ? place[p] : p;
-  }
-}
-
 // ---- checks ----
 
 int check_cache(const char* who, const hk_paged_cache* c) {
@@ -724,12 +743,14 @@ int hk_paged_compact(const hk_paged_cache* cache, int32_t* table_out, int32_t* r
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(paged_compact_kernel, dim3(1), dim3(kBook), 0, st, a);
   HK_TRY(launched("paged compact launch"));
-  const int64_t cells = (int64_t)cache->seqs * cache->table_width;
-  const int groups = (int)std::min<int64_t>((cells + 255) / 256, 1024);
-  hipLaunchKernelGGL(paged_rename_kernel, dim3(groups), dim3(256), 0, st, cache->table, table_out, cells, live_out,
-                     a.place, a.pages);
-  HK_TRY(launched("paged rename launch"));
-  hipLaunchKernelGGL(paged_move_kernel, dim3(kMoveGroups), dim3(256), 0, st, moves_of(cache, a.moves, a.count, true));
+  MoveArgs m = moves_of(cache, a.moves, a.count, true);
+  m.table = cache->table;
+  m.table_out = table_out;
+  m.live = live_out;
+  m.place = a.place;
+  m.cells = (int64_t)cache->seqs * cache->table_width;
+  m.pages = a.pages;
+  hipLaunchKernelGGL(paged_move_kernel, dim3(kMoveGroups), dim3(256), 0, st, m);
   return launched("paged move launch");
 }
 
