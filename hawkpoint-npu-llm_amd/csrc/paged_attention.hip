@@ -161,17 +161,21 @@ struct Run {
   int64_t begin, end, per;
   PlanPlace place;
   Entry entry;
+  PlanEven even;  // splits > 0: parts of equal length instead of runs
+  int task;       // of those, the workgroup's next task
 };
 
 // This workgroup's run; false: it has none.  Consecutive runs are on one XCD
 // (workgroups go round the eight), where they share K and V rows in its L2,
 // and the XCDs have equally many.
 constexpr int kXcds = 8;
+template <bool EVEN>
 __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape& s, int least, Run& run) {
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found_start;
   __shared__ int found[5];
   const int n = a.b.n;
+  run.even = {0, 0};
   // whether unit w per lies before `total`; sets the run's number and ends
   auto cut = [&](int64_t total) {
     run.per = plan_per(s, total, gridDim.x, least);
@@ -185,6 +189,14 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
     run.entry = load_entry(a, 0);
     if (!takes(a, run.entry.e.count)) return false;
     const int64_t head = plan_tiles(s, run.entry.e) == 1 ? plan_units(s, plan_span(s, run.entry.e, 0)) : wave_head_units(s, run.entry.e);
+    if constexpr (EVEN) {
+      run.even = plan_even(s, run.entry.e, s.heads * head, gridDim.x);
+      if (run.even.splits) {
+        run.w = (int)blockIdx.x % kXcds * ((int)gridDim.x / kXcds) + (int)blockIdx.x / kXcds;
+        run.task = run.w / run.even.splits;
+        return run.task < run.even.tasks;
+      }
+    }
     if (!cut(s.heads * head)) return false;
     run.place = wave_find(s, run.entry.e, 0, 0, run.begin);
     return true;
@@ -264,31 +276,57 @@ __device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShap
 struct Task {
   Entry entry;
   const int32_t* table;  // the sequence's pages
-  int64_t start;         // units before the task
-  int g, tile, r0, rows, pos0, blocks, kb0, kb1, seen;
+  int g, tile, r0, rows, pos0, kb0, kb1, seen;
   bool cut;
+  PlanParts parts;  // of a cut task
 };
+
+// Fills in t for blocks `mine` of the task of a kv head's tile.
+__device__ __forceinline__ void set_task(const PagedAttnArgs& a, const PlanShape& s, const Entry& entry, int head, int tile,
+                                         const PlanSpan& span, const PlanBlocks& mine, Task& t) {
+  t.entry = entry;
+  t.table = a.c.table + (int64_t)max(entry.seq, 0) * a.c.width;
+  t.g = head;
+  t.tile = tile;
+  t.r0 = tile * s.rows;
+  t.rows = min(s.rows, entry.e.count * a.group - t.r0);
+  t.pos0 = entry.e.length - entry.e.count;
+  t.kb0 = span.lo + mine.first;
+  t.kb1 = span.hi > span.lo ? span.lo + mine.end : t.kb0;
+  t.seen = span.seen;
+}
 
 // The task at the run's place, or the next one of which the run has blocks;
 // false: there is none.
+template <bool EVEN>
 __device__ __forceinline__ bool next_task(const PagedAttnArgs& a, const PlanShape& s, Run& run, Task& t) {
+  if (EVEN && run.even.splits) {
+    if (run.task >= run.even.tasks) return false;
+    const int tiles = plan_tiles(s, run.entry.e), head = uniform(run.task / tiles), tile = run.task - head * tiles;
+    const PlanSpan span = plan_span(s, run.entry.e, tile);
+    const int blocks = plan_blocks(span);
+    const PlanBlocks mine = plan_even_mine(blocks, run.even.splits, run.w - run.task * run.even.splits);
+    t.parts = {run.task * run.even.splits, plan_even_parts(blocks, run.even.splits)};
+    if (run.even.splits == 1) {
+      // (whole tasks: the workgroup's number plays no part)
+      set_task(a, s, run.entry, head, tile, span, {0, blocks}, t);
+      t.cut = false;
+    } else {
+      if (mine.first >= mine.end) return false;
+      set_task(a, s, run.entry, head, tile, span, mine, t);
+      t.cut = mine.end - mine.first < blocks;
+    }
+    run.task += run.even.splits == 1 ? (int)gridDim.x : run.even.tasks;
+    return true;
+  }
   for (; run.place.start < run.end; plan_next(a, s, run)) {
     const PlanSpan span = plan_span(s, run.entry.e, run.place.tile);
-    t.blocks = plan_blocks(span);
-    const PlanBlocks mine = plan_mine(s, run.place.start, t.blocks, run.begin, run.end);
+    const int blocks = plan_blocks(span);
+    const PlanBlocks mine = plan_mine(s, run.place.start, blocks, run.begin, run.end);
     if (mine.first >= mine.end) continue;
-    t.cut = mine.end - mine.first < t.blocks;
-    t.entry = run.entry;
-    t.table = a.c.table + (int64_t)max(run.entry.seq, 0) * a.c.width;
-    t.start = run.place.start;
-    t.g = run.place.head;
-    t.tile = run.place.tile;
-    t.r0 = run.place.tile * s.rows;
-    t.rows = min(s.rows, run.entry.e.count * a.group - t.r0);
-    t.pos0 = run.entry.e.length - run.entry.e.count;
-    t.kb0 = span.lo + mine.first;
-    t.kb1 = span.hi > span.lo ? span.lo + mine.end : t.kb0;
-    t.seen = span.seen;
+    set_task(a, s, run.entry, run.place.head, run.place.tile, span, mine, t);
+    t.cut = mine.end - mine.first < blocks;
+    t.parts = t.cut ? plan_parts(s, run.place.start, blocks, run.per) : PlanParts{0, 0};
     plan_next(a, s, run);
     return true;
   }
@@ -445,7 +483,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   const PlanShape shape = {a.c.kv_heads, a.group, a.by_group, a.window, N::kRows, kWaves * kNarrowSlots, kBlockCost, kNarrowTaskCost};
   Run run;
   Task t;
-  if (!plan_run(a, shape, 1, run) || !next_task(a, shape, run, t)) return;
+  if (!plan_run<false>(a, shape, 1, run) || !next_task<false>(a, shape, run, t)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, quad = lane >> 4;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
   char* const mylds = lds[wave];
@@ -624,7 +662,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            sv[n][h][r] = whole | sees(n, s0 + 16 * h + 4 * quad + r) ? sv[n][h][r] : -INFINITY;
+            sv[n][h][r] = (whole | sees(n, s0 + 16 * h + 4 * quad + r)) ? sv[n][h][r] : -INFINITY;
             mx = fmaxf(mx, sv[n][h][r]);
           }
         const float m_new = fmaxf(m_run[n], quad_max(mx) * ks), m_use = finite_max(m_new);
@@ -667,7 +705,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
 
     // the next task's first loads are under way while this one ends
     const Task done = t;
-    const bool more_tasks = next_task(a, shape, run, t);
+    const bool more_tasks = next_task<false>(a, shape, run, t);
     if (more_tasks) begin(t);
 
     // the waves' results meet: maxima and sums, then O through LDS 16 rows at a time
@@ -684,8 +722,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
       if (lane == 0) again[wave] = any;
     }
     const bool cut = done.cut;
-    const PlanParts done_parts = cut ? plan_parts(shape, done.start, done.blocks, run.per) : PlanParts{0, 0};
-    const int slot = plan_slot(done_parts, run.w) * (N::kPart * 4);
+    const int slot = plan_slot(done.parts, run.w) * (N::kPart * 4);
     constexpr int kPer = D / 16;  // outputs of a thread: dimensions kPer (tid % 16) .. of row tid / 16
     const int orow = tid >> 4, od = kPer * (tid & 15);
     bool note = false;
@@ -732,7 +769,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
     __syncthreads();  // the waves' V rows are free again
     if (!cut && note) rows_again<D, E4M3>(a, done.entry, g, r0, rows);
     if (cut) {
-      const Pending p = {done_parts, done.entry, g, done.tile};
+      const Pending p = {done.parts, done.entry, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     }
@@ -832,21 +869,19 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
 
 // ---- more rows: the waves share the rows ----
 //
-// A workgroup takes a tile of 128 QB rows, a wave 32 QB of them (QB columns of
+// A workgroup takes a tile of 128 rows, a wave 32 of them (the columns of
 // v_mfma_f32_32x32x16_bf16), and goes through the slots 64 at a time.  K and V
 // come through registers into two LDS buffers, a block ahead, one barrier per
-// block; a fragment of either serves QB products.  LDS reads bound the loop at
-// QB 1 (a fragment of 1 KiB per product of 32 cycles and wave is all that a CU
-// reads), so ...
+// block.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kWideSlots = 64;
 
-template <int D, int QB>
+template <int D>
 struct Wide {
-  static constexpr int kRows = 128 * QB;
+  static constexpr int kRows = 128;
   static constexpr int kBuf = kWideSlots * D;  // bf16 of one of K, V
   // floats of a part: O, max and sum per lane
-  static constexpr int kLaneFloats = QB * (D / 2 + 2);
+  static constexpr int kLaneFloats = D / 2 + 2;
   static constexpr int kPart = kThreads * kLaneFloats;
 };
 
@@ -872,50 +907,44 @@ __device__ __forceinline__ float half_sum(float v) {
 
 constexpr int wide_per_cu(int d) { return d == 64 ? 3 : 2; }
 
-template <int D, bool E4M3, int QB>
+template <int D, bool E4M3>
 __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(PagedAttnArgs a) {
-  using W = Wide<D, QB>;
+  using W = Wide<D>;
   constexpr int kRowBytes = D * (E4M3 ? 1 : 2), kLoads = kRowBytes / 64, kSteps = D / 16, kDims = D / 32;
-  constexpr int kAhead = 2;
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
   // of each 16 slots of a block: bit 0: they have a page, bit 1: an infinity or
   // NaN among the values, where not every row sees them all
   __shared__ __attribute__((aligned(16))) int note_lds[2][kWaves];
   __shared__ int last[2], again[kWaves];
-  constexpr int kQuads = D / 8;  // 16-byte words of a part's O per lane and QB
+  constexpr int kQuads = D / 8;  // 16-byte words of a part's O per lane
   const PlanShape shape = {a.c.kv_heads, a.group, a.by_group, a.window, W::kRows, kWideSlots, kBlockCost, kWideTaskCost};
   Run run;
   Task t;
-  if (!plan_run(a, shape, 4, run) || !next_task(a, shape, run, t)) return;
+  if (!plan_run<true>(a, shape, 4, run) || !next_task<true>(a, shape, run, t)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
   const int shift = a.c.page_shift, mask = (1 << shift) - 1;
   const __amdgpu_buffer_rsrc_t parts = parts_of(a);
   Pending pend[2];
   int pending = 0;
   // the finished rows of a tile, and their lse
-  auto finish = [&](const Entry& en, int g, int r0, int rows, const f32x16 (&o)[QB][kDims], const float (&ms)[QB], const float (&ls)[QB]) {
-    const float vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+  auto finish = [&](const Entry& en, int g, int r0, int rows, const f32x16 (&o)[kDims], float m, float l) {
+    const int at = 32 * wave + col;
+    if (at >= rows) return;
+    const int tok = plan_div(r0 + at, a.by_group), h = g * a.group + (r0 + at) - tok * a.group;
+    const int64_t row = en.row0 + tok;
+    const float f = l == 0.0f ? 0.0f : (E4M3 ? a.c.v_scale[g] : 1.0f) / l;
+    uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      const int at = 32 * (QB * wave + b) + col;
-      if (at >= rows) continue;
-      const int tok = plan_div(r0 + at, a.by_group), h = g * a.group + (r0 + at) - tok * a.group;
-      const int64_t row = en.row0 + tok;
-      const float l = ls[b], f = l == 0.0f ? 0.0f : vs / l;
-      uint16_t* dst = a.out + row * a.out_stride + h * D + 4 * half;
+    for (int d = 0; d < kDims; ++d)
 #pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x16& x = o[b][d];
-          u32x2_t y = {f32x2_to_bf16x2(x[4 * i] * f, x[4 * i + 1] * f), f32x2_to_bf16x2(x[4 * i + 2] * f, x[4 * i + 3] * f)};
-          if (l == 0.0f) y = u32x2_t{0u, 0u};
-          stg(reinterpret_cast<u32x2_t*>(dst + 32 * d + 8 * i), y);
-        }
-      if (a.lse && half == 0)
-        stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (ms[b] + __builtin_amdgcn_logf(l)) * kLn2);
-    }
+      for (int i = 0; i < 4; ++i) {
+        const f32x16& x = o[d];
+        u32x2_t y = {f32x2_to_bf16x2(x[4 * i] * f, x[4 * i + 1] * f), f32x2_to_bf16x2(x[4 * i + 2] * f, x[4 * i + 3] * f)};
+        if (l == 0.0f) y = u32x2_t{0u, 0u};
+        stg(reinterpret_cast<u32x2_t*>(dst + 32 * d + 8 * i), y);
+      }
+    if (a.lse && half == 0) stg(a.lse + row * a.q_heads + h, l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2);
   };
 
   // wave w loads slots 16 w .. of a block (one page's): resources that end
@@ -951,37 +980,29 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g, kb0 = t.kb0, kb1 = t.kb1;
     const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
     // the wave's rows [w0, w1) of the tile, and the positions they span
-    const int w0 = wave * 32 * QB, w1 = min(rows, w0 + 32 * QB);
+    const int w0 = wave * 32, w1 = min(rows, w0 + 32);
     const int wave_lo = pos0 + plan_div(r0 + w0, a.by_group), wave_hi = w1 > w0 ? pos0 + plan_div(r0 + w1 - 1, a.by_group) : -1;
     const int tile_lo = pos0 + plan_div(r0, a.by_group), tile_hi = pos0 + plan_div(r0 + rows - 1, a.by_group);
 
-    int pos[QB], low[QB];
-    bf16x8 qf[QB][kSteps];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      const int at = w0 + 32 * b + col, r = r0 + at, tok = plan_div(r, a.by_group);
+    int pos, low;  // (low, pos] are the slots that the lane's row sees
+    bf16x8 qf[kSteps];
+    {
+      const int at = w0 + col, r = r0 + at, tok = plan_div(r, a.by_group);
       const bool ok = at < rows;
-      pos[b] = ok ? pos0 + tok : -1;
-      low[b] = a.window > 0 ? pos[b] - a.window : -1;
+      pos = ok ? pos0 + tok : -1;
+      low = a.window > 0 ? pos - a.window : -1;
       const uint16_t* q = a.q + (t.entry.row0 + (ok ? tok : 0)) * a.q_stride + (g * a.group + (ok ? r - tok * a.group : 0)) * D;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) qf[b][s] = __builtin_bit_cast(bf16x8, load16(q + 16 * s + 8 * half));
+      for (int s = 0; s < kSteps; ++s) qf[s] = __builtin_bit_cast(bf16x8, load16(q + 16 * s + 8 * half));
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) settle(qf[s]);  // (before the loop, as in the narrow form)
     }
+    float m_run = -INFINITY, l_run = 0.0f;
+    f32x16 o[kDims];
 #pragma unroll
-    for (int b = 0; b < QB; ++b)
+    for (int d = 0; d < kDims; ++d)
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) settle(qf[b][s]);  // (before the loop, as in the narrow form)
-    float m_run[QB], l_run[QB];
-    f32x16 o[QB][kDims];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      m_run[b] = -INFINITY;
-      l_run[b] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
-    }
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
     // a block that every row of the tile sees whole (its pages apart)
     auto all_see = [&](int s0, int lo, int hi) {
@@ -1022,122 +1043,106 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
       if (kb + 1 < kb1) load_block(t, s0 + kWideSlots);
       if (s0 <= wave_hi) {
         const u32x4 notes = *reinterpret_cast<const u32x4*>(note_lds[buf]);
-        // S^T: lane holds slots 32 t + 8 (i / 4) + 4 half + i % 4 of row col.  The
-        // fragments of kAhead products are read while those before them run
-        // (left to itself the compiler reads one and waits for it)
-        f32x16 sv[QB][2];
+        // The block's products in order: S^T of slots 0 .. 31 and 32 .. 63 (kSteps
+        // each), then O^T with 16 slots' probabilities at a time (kDims each).
+        // Their left operands come from LDS two products ahead (left to itself
+        // the compiler reads one and waits for it).
+        constexpr int kQk = 2 * kSteps, kAll = kQk + 4 * kDims;
+        // S^T: lane holds slots 32 t + 8 (i / 4) + 4 half + i % 4 of row col; V: k
+        // index 8 half + e of product x stands for slot 16 x + 8 (e / 4) + 4 half
+        // + e % 4, the probabilities that this lane holds, and a group of 16 lanes
+        // reads 4 slots of 16 dimensions, transposed
+        f32x16 sv[2];
+        bf16x8 pf[4], left[2][2];
+        const int ra = 4 * half + ((lane & 15) >> 2), dd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        auto read_left = [&](int pair) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sv[b][t][i] = 0.0f;
-        {
-          bf16x8 kf[2][kAhead];
-          auto read_k = [&](int x) {  // fragments kAhead x ..: step % kSteps of slots 32 (step / kSteps) ..
-#pragma unroll
-            for (int y = 0; y < kAhead; ++y) {
-              const int r = 32 * ((kAhead * x + y) / kSteps) + col, s = (kAhead * x + y) % kSteps;
-              kf[x & 1][y] = *reinterpret_cast<const bf16x8*>(&ks_lds[buf][r * D + 8 * ((2 * s + half) ^ wide_k_key<D>(r))]);
-            }
-          };
-          read_k(0);
-#pragma unroll
-          for (int x = 0; x < 2 * kSteps / kAhead; ++x) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (x + 1 < 2 * kSteps / kAhead) read_k(x + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < kAhead; ++y)
-#pragma unroll
-              for (int b = 0; b < QB; ++b)
-                sv[b][(kAhead * x + y) / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    kf[x & 1][y], qf[b][(kAhead * x + y) % kSteps], sv[b][(kAhead * x + y) / kSteps], 0, 0, 0);
-          }
-        }
-        // bit h: slots 16 h .. of the block have a page
-        const int paged = uniform((int)((notes.x & 1) | (notes.y & 1) << 1 | (notes.z & 1) << 2 | (notes.w & 1) << 3));
-        const bool whole = all_see(s0, wave_lo, wave_hi) && paged == 15;
-        auto sees = [&](int b, int s) {
-          return (s <= pos[b]) & (s > low[b]) & (bool)((paged >> ((s >> 4) & 3)) & 1);
-        };
-        if (!whole) {
-#pragma unroll
-          for (int b = 0; b < QB; ++b)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                sv[b][t][i] = sees(b, s0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) ? sv[b][t][i] : -INFINITY;
-        }
-        bf16x8 pf[QB][4];
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sv[b][t][i]);
-          const float m_new = fmaxf(m_run[b], half_max(mx) * ks), m_use = finite_max(m_new);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_use);
-          float rs = 0.0f;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              sv[b][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[b][t][i], ks, -m_use));
-              rs += sv[b][t][i];
-            }
-          l_run[b] = l_run[b] * alpha + rs;
-          m_run[b] = m_new;
-          if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) o[b][d] *= alpha;
-          }
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            u32x4 pw;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              pw[e] = f32x2_to_bf16x2(sv[b][t >> 1][8 * (t & 1) + 2 * e], sv[b][t >> 1][8 * (t & 1) + 2 * e + 1]);
-            pf[b][t] = __builtin_bit_cast(bf16x8, pw);
-          }
-        }
-        if (!whole) poison |= (notes.x | notes.y | notes.z | notes.w) & 2;
-        {
-          // k index 8 half + e of product t stands for slot 16 t + 8 (e / 4) +
-          // 4 half + e % 4, the probabilities this lane holds; a group of 16
-          // lanes reads 4 slots of 16 dimensions, transposed
-          const int ra = 4 * half + ((lane & 15) >> 2), dd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          bf16x8 vf[2][kAhead];
-          auto read_v = [&](int x) {  // fragments kAhead x ..: dimensions 32 (step % kDims) .. of slots 16 (step / kDims) ..
-#pragma unroll
-            for (int y = 0; y < kAhead; ++y) {
-              const int t = (kAhead * x + y) / kDims, d = (kAhead * x + y) % kDims;
-              const int r1 = 16 * t + ra, r2 = r1 + 8, dim = 32 * d + dd;
+          for (int y = 0; y < 2; ++y) {
+            const int x = 2 * pair + y;
+            if (x < kQk) {
+              const int r = 32 * (x / kSteps) + col, s = x % kSteps;
+              left[pair & 1][y] = *reinterpret_cast<const bf16x8*>(&ks_lds[buf][r * D + 8 * ((2 * s + half) ^ wide_k_key<D>(r))]);
+            } else {
+              const int d = (x - kQk) % kDims, r1 = 16 * ((x - kQk) / kDims) + ra, r2 = r1 + 8, dim = 32 * d + dd;
               const v4s16 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                   (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r1 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r1)) + (dim & 7)]);
               const v4s16 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                   (__attribute__((address_space(3))) v4s16*)&vs_lds[buf][r2 * D + 8 * ((dim >> 3) ^ wide_v_key<D>(r2)) + (dim & 7)]);
               const u32x2_t w0 = __builtin_bit_cast(u32x2_t, t0), w1 = __builtin_bit_cast(u32x2_t, t1);
-              vf[x & 1][y] = __builtin_bit_cast(bf16x8, u32x4{w0.x, w0.y, w1.x, w1.y});
-            }
-          };
-          read_v(0);
-#pragma unroll
-          for (int x = 0; x < 4 * kDims / kAhead; ++x) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (x + 1 < 4 * kDims / kAhead) read_v(x + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < kAhead; ++y) {
-              const int t = (kAhead * x + y) / kDims, d = (kAhead * x + y) % kDims;
-#pragma unroll
-              for (int b = 0; b < QB; ++b)
-                o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 1][y], pf[b][t], o[b][d], 0, 0, 0);
+              left[pair & 1][y] = __builtin_bit_cast(bf16x8, u32x4{w0.x, w0.y, w1.x, w1.y});
             }
           }
+        };
+        auto products = [&](auto from, auto count) {
+#pragma unroll
+          for (int x = from; x < from + count; ++x) {
+            if (x % 2 == 0) {
+              __builtin_amdgcn_sched_barrier(0);
+              if (x + 2 < kAll) read_left(x / 2 + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const bf16x8 l = left[(x / 2) & 1][x % 2];
+            if (x < kQk)
+              sv[x / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l, qf[x % kSteps], sv[x / kSteps], 0, 0, 0);
+            else
+              o[(x - kQk) % kDims] =
+                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(l, pf[(x - kQk) / kDims], o[(x - kQk) % kDims], 0, 0, 0);
+          }
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sv[h][i] = 0.0f;
+
+        // bit h: slots 16 h .. of the block have a page
+        const int paged = uniform((int)((notes.x & 1) | (notes.y & 1) << 1 | (notes.z & 1) << 2 | (notes.w & 1) << 3));
+        const bool whole = all_see(s0, wave_lo, wave_hi) && paged == 15;
+        if (!whole) poison |= (notes.x | notes.y | notes.z | notes.w) & 2;
+        auto hide = [&](int h) {
+          if (whole) return;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int s = s0 + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
+            const bool sees = (s <= pos) & (s > low) & (bool)((paged >> ((s >> 4) & 3)) & 1);  // (no branches: the lanes differ)
+            sv[h][i] = sees ? sv[h][i] : -INFINITY;
+          }
+        };
+        using Qk = std::integral_constant<int, kQk>;
+        __builtin_amdgcn_s_setprio(1);  // (a wave in its products goes before one in its softmax)
+        read_left(0);
+        products(std::integral_constant<int, 0>(), Qk());
+        __builtin_amdgcn_s_setprio(0);
+        hide(0);
+        hide(1);
+        float mx = fmaxf(sv[0][0], sv[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(fmaxf(mx, sv[0][i]), sv[1][i]);
+        const float m_new = fmaxf(m_run, half_max(mx) * ks), m_use = finite_max(m_new);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        m_run = m_new;
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          u32x4 pw;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[x / 2][8 * (x % 2) + 2 * i], ks, -m_use));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[x / 2][8 * (x % 2) + 2 * i + 1], ks, -m_use));
+            sum += e0;
+            sum += e1;
+            pw[i] = f32x2_to_bf16x2(e0, e1);
+          }
+          pf[x] = __builtin_bit_cast(bf16x8, pw);
         }
+        l_run = l_run * alpha + sum;
+        // once the running maxima settle, alpha is 1 in every lane
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[d] *= alpha;
+        }
+        __builtin_amdgcn_s_setprio(1);
+        products(Qk(), std::integral_constant<int, 4 * kDims>());
+        __builtin_amdgcn_s_setprio(0);
       }
       if (kb + 1 < kb1) {
         find_page(t, s0 + 2 * kWideSlots);
@@ -1147,34 +1152,28 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
 
     // the next task's first loads are under way while this one ends
     const Task done = t;
-    const bool more_tasks = next_task(a, shape, run, t);
+    const bool more_tasks = next_task<true>(a, shape, run, t);
     if (more_tasks) begin(t);
     const bool cut = done.cut;
-    const PlanParts done_parts = cut ? plan_parts(shape, done.start, done.blocks, run.per) : PlanParts{0, 0};
-#pragma unroll
-    for (int b = 0; b < QB; ++b) l_run[b] = half_sum(l_run[b]);
+    l_run = half_sum(l_run);
     if (lane == 0) again[wave] = poison;
     __syncthreads();  // the buffers have been read
     const bool note = again[0] | again[1] | again[2] | again[3];
     if (cut) {
       // parts lie lane by lane: word i of thread t at 16 (i threads + t) bytes
-      const int slot = plan_slot(done_parts, run.w) * (W::kPart * 4);
+      const int slot = plan_slot(done.parts, run.w) * (W::kPart * 4);
       if (wave_hi >= 0) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-#pragma unroll
-          for (int i = 0; i < kQuads; ++i) {
-            const f32x16& x = o[b][i / 4];
-            const f32x4 y = {x[4 * (i % 4)], x[4 * (i % 4) + 1], x[4 * (i % 4) + 2], x[4 * (i % 4) + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts,
-                                                   slot + 16 * (kThreads * (b * kQuads + i) + tid), 0, kSc1);
-          }
-          // (a NaN in the place of a maximum, which none is, passes the note on)
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(note ? NAN : m_run[b]), __float_as_uint(l_run[b])}, parts,
-                                                slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
+        for (int i = 0; i < kQuads; ++i) {
+          const f32x16& x = o[i / 4];
+          const f32x4 y = {x[4 * (i % 4)], x[4 * (i % 4) + 1], x[4 * (i % 4) + 2], x[4 * (i % 4) + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, slot + 16 * (kThreads * i + tid), 0, kSc1);
         }
+        // (a NaN in the place of a maximum, which none is, passes the note on)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(note ? NAN : m_run), __float_as_uint(l_run)}, parts,
+                                              slot + 16 * kThreads * kQuads + 8 * tid, 0, kSc1);
       }
-      const Pending p = {done_parts, done.entry, g, done.tile};
+      const Pending p = {done.parts, done.entry, g, done.tile};
       if (pending == 0) pend[0] = p; else pend[1] = p;
       ++pending;
     } else if (note) {
@@ -1193,39 +1192,31 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     const PlanParts pp = p.parts;
     const int r0 = p.tile * W::kRows, rows = min(W::kRows, p.entry.e.count * a.group - r0);
     // (a wave whose rows stand at negative positions has no part)
-    const bool has = p.entry.e.length - p.entry.e.count + plan_div(r0 + min(rows, 32 * QB * (wave + 1)) - 1, a.by_group) >= 0 &&
-                     rows > 32 * QB * wave;
-    float m[QB], l[QB];
-    f32x16 o[QB][kDims];
+    const bool has = p.entry.e.length - p.entry.e.count + plan_div(r0 + min(rows, 32 * (wave + 1)) - 1, a.by_group) >= 0 &&
+                     rows > 32 * wave;
+    float m = -INFINITY, l = 0.0f;
+    f32x16 o[kDims];
     bool note = false;
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      m[b] = -INFINITY;
-      l[b] = 0.0f;
+    for (int d = 0; d < kDims; ++d)
 #pragma unroll
-      for (int d = 0; d < kDims; ++d)
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    for (int k = 0; has && k < pp.count; ++k) {
+      const int slot = plan_slot(pp, pp.first + k) * (W::kPart * 4);
+      const u32x2_t ml = __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * kQuads + 8 * tid, 0, kSc1);
+      u32x4 y[kQuads];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
-      if (!has) continue;
-      for (int k = 0; k < pp.count; ++k) {
-        const int slot = plan_slot(pp, pp.first + k) * (W::kPart * 4);
-        const u32x2_t ml =
-            __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * QB * kQuads + 8 * (kThreads * b + tid), 0, kSc1);
-        u32x4 y[kQuads];
+      for (int i = 0; i < kQuads; ++i)
+        y[i] = __builtin_amdgcn_raw_buffer_load_b128(parts, slot + 16 * (kThreads * i + tid), 0, kSc1);
+      const float mk = __uint_as_float(ml.x), m_new = fmaxf(m, mk);
+      const float f0 = __builtin_amdgcn_exp2f(m - finite_max(m_new)), f1 = __builtin_amdgcn_exp2f(mk - finite_max(m_new));
+      note |= mk != mk;
+      l = l * f0 + __uint_as_float(ml.y) * f1;
+      m = m_new;
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i)
-          y[i] = __builtin_amdgcn_raw_buffer_load_b128(parts, slot + 16 * (kThreads * (b * kQuads + i) + tid), 0, kSc1);
-        const float mk = __uint_as_float(ml.x), m_new = fmaxf(m[b], mk);
-        const float f0 = __builtin_amdgcn_exp2f(m[b] - finite_max(m_new)), f1 = __builtin_amdgcn_exp2f(mk - finite_max(m_new));
-        note |= mk != mk;
-        l[b] = l[b] * f0 + __uint_as_float(ml.y) * f1;
-        m[b] = m_new;
+      for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            o[b][i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[i][c]), f1, o[b][i / 4][4 * (i % 4) + c] * f0);
-      }
+        for (int c = 0; c < 4; ++c) o[i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[i][c]), f1, o[i / 4][4 * (i % 4) + c] * f0);
     }
     const int any = __any(note);
     if (lane == 0) again[wave] = any;
@@ -1240,14 +1231,13 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
 
 // Launches: as many workgroups as the GPU holds at once.
 constexpr int kCus = 256;
-constexpr int kWideQB = 1;
 constexpr bool fits(long long groups, long long part) {
   return groups <= kPagedTicketWords && groups % 8 == 0 &&
          4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
 }
 static_assert(fits(4 * kCus, Narrow<64, false, 1>::kPart) && fits(3 * kCus, Narrow<128, true, 1>::kPart) &&
-                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kCus * wide_per_cu(128), Wide<128, kWideQB>::kPart) &&
-                  fits(kCus * wide_per_cu(64), Wide<64, kWideQB>::kPart),
+                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kCus * wide_per_cu(128), Wide<128>::kPart) &&
+                  fits(kCus * wide_per_cu(64), Wide<64>::kPart),
               "partial results and tickets fit the workspace");
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
@@ -1275,7 +1265,7 @@ void launch(PagedAttnArgs a, hipStream_t stream) {
     a.rows_min = few + 1;
     narrow<D, E4M3>(b, few, stream);
   }
-  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3, kWideQB>), dim3(kCus * wide_per_cu(D)), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3>), dim3(kCus * wide_per_cu(D)), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace

@@ -138,4 +138,33 @@ HK_PLAN PlanParts plan_parts(const PlanShape& s, int64_t start, int blocks, int6
 }
 HK_PLAN int plan_slot(const PlanParts& p, int w) { return 2 * w + (w == p.first ? 1 : 0); }
 
+// A batch of one entry over a long context may be cut another way: every task
+// into `splits` parts of as many blocks each (or, of more tasks than
+// workgroups, whole tasks dealt out one after the other), so that the
+// workgroups of a kv head go through the same slots at the same time and find
+// them in their XCD's L2.  Equal runs start all over the context: a context that
+// L2 does not hold then comes from memory once for each tile.
+struct PlanEven {
+  int splits;  // 0: equal runs
+  int tasks;
+};
+// Taken where the longest workgroup has at most a quarter more than the average
+// (an entry without a past has tiles of one block and of all: half the
+// workgroups would wait).  `total`: units of all tasks.
+HK_PLAN PlanEven plan_even(const PlanShape& s, const PlanEntry& e, int64_t total, int groups) {
+  const int tiles = plan_tiles(s, e), tasks = s.heads * tiles;
+  const int splits = tasks <= groups ? groups / tasks : 1, rounds = (tasks + groups - 1) / groups;
+  const int blocks = plan_blocks(plan_span(s, e, tiles - 1));
+  const int64_t longest = rounds * (s.task_cost + (int64_t)s.block_cost * ((blocks + splits - 1) / splits));
+  return {4 * longest * groups <= 5 * total ? splits : 0, tasks};
+}
+
+// Part `part` of `splits` of a task's blocks, and the parts that have some.
+HK_PLAN int plan_even_parts(int blocks, int splits) { return blocks < splits ? blocks : splits; }
+HK_PLAN PlanBlocks plan_even_mine(int blocks, int splits, int part) {
+  const int parts = plan_even_parts(blocks, splits);
+  if (part >= parts) return {0, 0};
+  return {(int)((int64_t)blocks * part / parts), (int)((int64_t)blocks * (part + 1) / parts)};
+}
+
 }  // namespace hk

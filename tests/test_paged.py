@@ -307,6 +307,25 @@ int main() {
         }
       }
     CHECK(tasks == got.size());
+    // the even cut of each entry by itself
+    for (auto& x : e) {
+      if (!x.count) continue;
+      const PlanEven even = plan_even(s, x, s.heads * plan_head_units(s, x), groups);
+      if (!even.splits) continue;
+      const int tiles = plan_tiles(s, x);
+      CHECK(even.tasks == s.heads * tiles && (even.splits == 1 || even.splits * even.tasks <= groups));
+      for (int task = 0; task < even.tasks; ++task) {
+        const int blocks = plan_blocks(plan_span(s, x, task % tiles)), parts = plan_even_parts(blocks, even.splits);
+        int next = 0;
+        for (int part = 0; part < even.splits; ++part) {
+          const PlanBlocks mine = plan_even_mine(blocks, even.splits, part);
+          CHECK((mine.first < mine.end) == (part < parts));
+          if (part < parts) CHECK(mine.first == next);
+          if (part < parts) next = mine.end;
+        }
+        CHECK(next == blocks && parts >= 1);
+      }
+    }
   }
 }
 """
