@@ -301,6 +301,123 @@ def test_attention_ignores_what_a_row_does_not_see(hk_lib, dim, e4m3, counts, wi
     check_attention(got[keep], lse[keep], raw[keep], tuple(w[keep] for w in want), _floats(q)[keep], cache, 0.1)
 
 
+def test_attention_of_a_poisoned_long_sequence(hk_lib):
+    """One entry whose tiles are split over workgroups: the note of a NaN that only the last row sees comes with the
+    parts."""
+    announce("paged attention: poisoned slots of a sequence that is split")
+    rng = np.random.default_rng(14)
+    cache = Cache(rng, pages=160, kv_heads=2, page=16, dim=128, seqs=1, width=160)
+    cache.give([2400], rng)
+    cache.fill(rng)
+    page = cache.o["table"][0, 2399 // 16]
+    cache.o["v"][0, page, 1, 2399 % 16, 9] = np.nan
+    cache.upload()
+    q = _bits(rng.normal(size=(70, 4, 128)))
+    want = oracle.attention(cache.o, 0, _floats(q), [0], [0, 70], 0.1)
+    got = attention(cache, 0, q, [0], [0, 70], scale=0.1)
+    assert np.isnan(want[0]).sum() == 2  # the last row's two heads of the second kv head
+    check_attention(*got, want, _floats(q), cache, 0.1)
+
+
+@pytest.mark.parametrize("dim,e4m3,entries", [
+    (64, False, [(2500, 150)]), (128, False, [(3000, 90)]), (128, True, [(2600, 200)]), (64, True, [(1700, 300)]),
+    (128, False, [(700, 700)]), (64, False, [(1500, 40), (1500, 41)])])
+def test_attention_of_long_pieces(hk_lib, dim, e4m3, entries):
+    """Tiles cut into equal parts, and into runs."""
+    announce(f"paged attention: long pieces, dim {dim}, e4m3 {e4m3}, {entries}")
+    rng = np.random.default_rng(dim + len(entries))
+    need = sum(-(-n // 32) for n, _ in entries)
+    cache = Cache(rng, layers=2, pages=need + 2, kv_heads=2, page=32, dim=dim, seqs=len(entries), width=need, e4m3=e4m3)
+    cache.give([n for n, _ in entries], rng)
+    for layer in (0, 1):
+        cache.fill(rng, layer)
+    cache.upload()
+    first = np.cumsum([0] + [c for _, c in entries])
+    q = _bits(rng.normal(size=(first[-1], 6, dim)))
+    for layer in (0, 1):
+        got = attention(cache, layer, q, range(len(entries)), first, scale=0.1)
+        want = oracle.attention(cache.o, layer, _floats(q), range(len(entries)), first, 0.1)
+        check_attention(*got, want, _floats(q), cache, 0.1)
+
+
+def test_attention_of_more_tasks_than_workgroups(hk_lib):
+    """32 kv heads of 25 tiles: whole tasks dealt out in rounds; with a second, empty entry, equal runs."""
+    announce("paged attention: 800 tasks")
+    rng = np.random.default_rng(31)
+    cache = Cache(rng, pages=80, kv_heads=32, page=16, dim=64, seqs=2, width=80)
+    cache.give([1200], rng)
+    cache.fill(rng)
+    cache.upload()
+    q = _bits(rng.normal(size=(800, 128, 64)))
+    calls = [attention(cache, 0, q, [0], [0, 800], scale=0.125), attention(cache, 0, q, [0, 1], [0, 800, 800], scale=0.125)]
+    for g in (0, 17, 31):
+        part = dict(cache.o, k=cache.o["k"][:, :, g:g + 1], v=cache.o["v"][:, :, g:g + 1])
+        mine = slice(4 * g, 4 * g + 4)
+        rows = np.arange(0, 800, 7)
+        # (the oracle goes row by row: a seventh of them, each an entry of its own length)
+        want = [np.concatenate(w) for w in zip(*(
+            oracle.attention(dict(part, length=np.array([401 + t, 0], np.int32)), 0, _floats(q[t:t + 1, mine]), [0], [0, 1],
+                             0.125) for t in rows))]
+        for out, lse, raw in calls:
+            check_attention(out[rows][:, mine], lse[rows][:, mine], raw[rows][:, mine], want, _floats(q[rows][:, mine]), cache,
+                            0.125)
+
+
+@pytest.mark.parametrize("n,counts", [(257, (1, 1, 1)), (700, (0, 1, 2)), (700, (1, 40, 0)), (4096, (1, 0, 1))])
+def test_attention_of_many_entries(hk_lib, n, counts):
+    """More entries than a workgroup has threads; sequences in any order, some in several entries."""
+    announce(f"paged attention: {n} entries")
+    rng = np.random.default_rng(n)
+    cache = Cache(rng, pages=120, kv_heads=1, page=16, dim=64, seqs=40, width=4)
+    cache.give(list(rng.integers(1, 49, 40)), rng)
+    cache.fill(rng)
+    cache.upload()
+    seqs = rng.integers(0, 40, n)
+    per = [counts[i % 3] for i in range(n)]
+    first = np.cumsum([0] + per)
+    q = _bits(rng.normal(size=(first[-1], 2, 64)))
+    got = attention(cache, 0, q, seqs, first, scale=0.125)
+    rows = np.unique(rng.integers(0, first[-1], 400))
+    want = oracle.attention(cache.o, 0, _floats(q), seqs, first, 0.125)
+    check_attention(*(x[rows] for x in got), tuple(w[rows] for w in want), _floats(q)[rows], cache, 0.125)
+
+
+def test_attention_on_two_streams(hk_lib):
+    """Calls in flight at once on streams of their own, each with its workspace; then the same stream after stream."""
+    from runtime import hip, paged
+
+    announce("paged attention: two streams")
+    rng = np.random.default_rng(41)
+    streams, sides = [], []
+    for i in range(2):
+        handle = ctypes.c_void_p()
+        hip.check(hk_lib.hk_stream_create(ctypes.byref(handle)), "hk_stream_create")
+        streams.append(handle.value)
+        cache = Cache(rng, pages=400, kv_heads=2, page=16, dim=64, seqs=3, width=200)
+        cache.give([3000, 1500, 200], rng)
+        cache.fill(rng)
+        cache.upload()
+        first = np.array([0, 1, 2, 3 + 90 * i])
+        q = _bits(rng.normal(size=(first[-1], 4, 64)))
+        sides.append((cache, q, first, oracle.attention(cache.o, 0, _floats(q), [0, 1, 2], first, 0.125)))
+    bufs = []
+    for cache, q, first, _ in sides:
+        bufs.append((_dev(q), _dev(first.astype(np.int32)), _dev(np.zeros(q.shape, np.uint16)),
+                     _dev(np.zeros(q.shape[:2], np.float32))))
+    _sync()
+    for _ in range(20):
+        for stream, (cache, q, first, _), (Q, F, O, L) in zip(streams, sides, bufs):
+            hip.check(paged.lib().hk_paged_attention(
+                ctypes.byref(cache.c), 0, Q.ptr, 256, None, F.ptr, 3, len(q), int(np.diff(first).max()), 4, 0.125, 0, O.ptr, 256,
+                L.ptr, cache.bufs["workspace"].ptr, stream), "hk_paged_attention")
+    for stream, (cache, q, first, want), (Q, F, O, L) in zip(streams, sides, bufs):
+        hip.check(hk_lib.hk_stream_sync(stream), "sync")
+        raw = O.read(np.uint16, q.size).reshape(q.shape)
+        check_attention(_floats(raw), L.read(np.float32, q[:, :, 0].size).reshape(q.shape[:2]), raw, want, _floats(q), cache, 0.125)
+    for stream in streams:
+        hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")
+
+
 def test_attention_layers_and_far_pages(hk_lib):
     """Layers of their own, and pages more than 4 GiB into the pool."""
     from runtime import hip
@@ -593,6 +710,88 @@ def test_fork_and_compact_sizes(hk_lib, pages, seqs):
 
 
 # ---- together ----
+
+
+class Graph:
+    """A stream's work between ``with`` and its end, captured and replayed through the HIP runtime of libhk.so."""
+
+    def __init__(self, stream):
+        # the runtime that libhk.so is bound to is in the process already: its functions by their global names
+        path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+        self.hip, self.stream = ctypes.CDLL(path), ctypes.c_void_p(stream)
+        self.graph, self.exe = ctypes.c_void_p(), ctypes.c_void_p()
+
+    def _ok(self, rc):
+        assert rc == 0, rc
+
+    def __enter__(self):
+        self._ok(self.hip.hipStreamBeginCapture(self.stream, 0))
+
+    def __exit__(self, kind, *_):
+        self._ok(self.hip.hipStreamEndCapture(self.stream, ctypes.byref(self.graph)))
+        if kind is None:
+            self._ok(self.hip.hipGraphInstantiate(ctypes.byref(self.exe), self.graph, None, None, ctypes.c_size_t(0)))
+
+    def replay(self):
+        self._ok(self.hip.hipGraphLaunch(self.exe, self.stream))
+
+    def close(self):
+        self._ok(self.hip.hipGraphExecDestroy(self.exe))
+        self._ok(self.hip.hipGraphDestroy(self.graph))
+
+
+@pytest.mark.parametrize("dim,e4m3", [(64, False), (128, True)])
+def test_a_captured_step_serves_every_later_length(hk_lib, dim, e4m3):
+    """Fork, append and attention of one decode step in a graph: each replay goes on from the lengths that the one
+    before left on the device, over page ends and past lengths that cut the work in other places, with eager calls and
+    synchronisations between the replays."""
+    from runtime import hip, paged
+
+    announce(f"paged cache: captured step, dim {dim}, e4m3 {e4m3}")
+    rng = np.random.default_rng(51)
+    hq, hkv, page, seqs, width = 6, 2, 16, 3, 40
+    cache = Cache(rng, pages=110, kv_heads=hkv, page=page, dim=dim, seqs=seqs, width=width, e4m3=e4m3, poison=False)
+    cache.give([30, 599, 15], rng)
+    cache.fill(rng)
+    cache.upload()
+    handle = ctypes.c_void_p()
+    hip.check(hk_lib.hk_stream_create(ctypes.byref(handle)), "hk_stream_create")
+    stream = handle.value
+    cos, sin = _tables(width * page, dim, rng)
+    C, S, ONE = _dev(cos), _dev(sin), _dev(np.ones(seqs, np.int32))
+    FIRST, STATUS = _dev(np.arange(seqs + 1, dtype=np.int32)), _dev(np.zeros(2, np.int32))
+    IN, Q = hip.DeviceBuffer(2 * seqs * (hq + 2 * hkv) * dim), hip.DeviceBuffer(2 * seqs * hq * dim)
+    OUT, LSE = hip.DeviceBuffer(2 * seqs * hq * dim), hip.DeviceBuffer(4 * seqs * hq)
+    _sync()
+    lib, c, ws = paged.lib(), ctypes.byref(cache.c), cache.bufs["workspace"].ptr
+    graph = Graph(stream)
+    with graph:
+        hip.check(lib.hk_paged_fork(c, None, None, None, ONE.ptr, seqs, STATUS.ptr, ws, stream), "hk_paged_fork")
+        hip.check(lib.hk_paged_append(c, 0, IN.ptr, (hq + 2 * hkv) * dim, C.ptr, S.ptr, width * page, None, FIRST.ptr, seqs,
+                                      seqs, hq, Q.ptr, hq * dim, stream), "hk_paged_append")
+        hip.check(lib.hk_paged_attention(c, 0, Q.ptr, hq * dim, None, FIRST.ptr, seqs, seqs, 1, hq, dim**-0.5, 0, OUT.ptr,
+                                         hq * dim, LSE.ptr, ws, stream), "hk_paged_attention")
+    for step in range(6):
+        x = _bits(rng.normal(size=(seqs, hq + 2 * hkv, dim)))
+        IN.write(x)
+        graph.replay()
+        hip.check(hk_lib.hk_stream_sync(stream), "sync")
+        n = [int(v) for v in cache.o["length"]]
+        assert tuple(STATUS.read(np.int32, 2)) == oracle.fork(cache.o, [0, 1, 2], [0, 1, 2], n, [1] * 3) == (0, 0)
+        oracle.append(cache.o, 0, _floats(x), [0, 1, 2], [0, 1, 2, 3], hq, cos, sin, cache.store(0))
+        # (a key at a rounding border may be its neighbour: the attention is checked on what the pool holds)
+        for y in "kv":
+            cache.o[y][0] = cache.decode(cache.download(y, 0), y, 0)
+        q = _floats(Q.read(np.uint16, seqs * hq * dim).reshape(seqs, hq, dim))
+        raw = OUT.read(np.uint16, seqs * hq * dim).reshape(seqs, hq, dim)
+        lse = LSE.read(np.float32, seqs * hq).reshape(seqs, hq)
+        want = oracle.attention(cache.o, 0, q, [0, 1, 2], [0, 1, 2, 3], dim**-0.5)
+        check_attention(_floats(raw), lse, raw, want, q, cache, dim**-0.5)
+        # the eager call on the same inputs gives the same bits
+        again = attention(cache, 0, _bits(q), [0, 1, 2], [0, 1, 2, 3], scale=dim**-0.5)
+        np.testing.assert_array_equal(again[2], raw)
+    graph.close()
+    hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")
 
 
 def test_chats_share_a_prompt(hk_lib):
