@@ -621,6 +621,10 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
     return fail("hk_paged_append: the RoPE tables must be aligned to 16 bytes");
   if (rope_cos && positions < (int64_t)cache->table_width * cache->page_size)
     return fail("hk_paged_append: RoPE tables shorter than the longest sequence");
+  if (tokens >= 1 << 24) {  // (a launch has 2^32 threads at most)
+    set_error("hk_paged_append: 2^24 tokens or more in a call");
+    return HK_ERR_UNSUPPORTED;
+  }
   if (n == 0 || tokens == 0) return 0;
   AppendArgs a = {pool_of(cache, layer), {seqs, first, n, tokens}, qkv, q_out, rope_cos, rope_sin, qkv_stride,
                   q_out_stride, q_heads};
@@ -651,10 +655,11 @@ int hk_paged_attention(const hk_paged_cache* cache, int32_t layer, const uint16_
   HK_TRY(check_rows(who, "out", out, out_stride, width));
   HK_TRY(check_workspace(who, workspace));
   if (max_new < 1) return fail("hk_paged_attention: max_new must be positive");
-  if ((int64_t)tokens * q_heads > INT32_MAX) {
-    set_error("hk_paged_attention: more than 2^31 - 1 rows (tokens x q_heads)");
+  if ((int64_t)tokens * q_heads > INT32_MAX / 2) {
+    set_error("hk_paged_attention: more than 2^30 rows (tokens x q_heads)");
     return HK_ERR_UNSUPPORTED;
   }
+  if (out == q && out_stride != q_stride) return fail("hk_paged_attention: in place only with equal strides");
   if (window < 0) return fail("hk_paged_attention: negative window");
   if (!std::isfinite(scale) || !(scale > 0.0f)) return fail("hk_paged_attention: scale must be finite and positive");
   if (n == 0 || tokens == 0) return 0;

@@ -336,6 +336,13 @@ __device__ __forceinline__ bool next_task(const PagedAttnArgs& a, const PlanShap
 // 2^(score - max): where all scores are -inf the maximum is no number to subtract.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// What a product q . k is multiplied by, for powers of two.  Not zero where
+// tiny factors underflow: a hidden score is -inf times it.
+template <bool E4M3>
+__device__ __forceinline__ float score_scale(const PagedAttnArgs& a, int g) {
+  return fmaxf((E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e, __builtin_bit_cast(float, 1u));
+}
+
 // Whether one of the eight bf16 values is an infinity or NaN.
 __device__ __forceinline__ bool not_finite(const u32x4& v) {
   bool bad = false;
@@ -402,7 +409,7 @@ __device__ __forceinline__ void rows_again(const PagedAttnArgs& a, const Entry& 
   constexpr int kPer = D / 64;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), shift = a.c.page_shift;
   const int32_t* const table = a.c.table + (int64_t)max(en.seq, 0) * a.c.width;
-  const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e, vs = E4M3 ? a.c.v_scale[g] : 1.0f;
+  const float ks = score_scale<E4M3>(a, g), vs = E4M3 ? a.c.v_scale[g] : 1.0f;
   for (int r = r0 + wave; r < r0 + rows; r += kWaves) {
     const int tok = plan_div(r, a.by_group), h = g * a.group + r - tok * a.group, p = en.e.length - en.e.count + tok;
     const int64_t row = en.row0 + tok;
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_na
   begin(t);
   for (;;) {
     const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g;
-    const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
+    const float ks = score_scale<E4M3>(a, g);
 
     // this lane's rows: position, and Q as the right operand (row col of each
     // group, dimensions as the K loads give them)
@@ -981,7 +988,7 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
   begin(t);
   for (;;) {
     const int r0 = t.r0, rows = t.rows, pos0 = t.pos0, g = t.g, kb0 = t.kb0, kb1 = t.kb1;
-    const float ks = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
+    const float ks = score_scale<E4M3>(a, g);
     // the wave's rows [w0, w1) of the tile, and the positions they span
     const int w0 = wave * 32, w1 = min(rows, w0 + 32);
     const int wave_lo = pos0 + plan_div(r0 + w0, a.by_group), wave_hi = w1 > w0 ? pos0 + plan_div(r0 + w1 - 1, a.by_group) : -1;
@@ -1304,15 +1311,17 @@ static_assert(fits(4 * kCus, Narrow<64, false, 1>::kPart) && fits(3 * kCus, Narr
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
 // most as far as the caller knows.
 template <int D, bool E4M3>
-void narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
+int narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
   if (rows <= 16)
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kCus * narrow_per_cu(D, E4M3, 1)), dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kCus * narrow_per_cu(D, E4M3, 2)), dim3(kThreads), 0, stream, a);
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
 }
 
 template <int D, bool E4M3>
-void launch(PagedAttnArgs a, hipStream_t stream) {
+int launch(PagedAttnArgs a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_new * a.group;
   a.by_group = plan_divisor(a.group);
   a.rows_min = 1;
@@ -1324,21 +1333,19 @@ void launch(PagedAttnArgs a, hipStream_t stream) {
     PagedAttnArgs b = a;
     b.rows_max = few;
     a.rows_min = few + 1;
-    narrow<D, E4M3>(b, few, stream);
+    if (const int rc = narrow<D, E4M3>(b, few, stream)) return rc;
   }
   hipLaunchKernelGGL((paged_wide_kernel<D, E4M3>), dim3(kCus * wide_per_cu(D)), dim3(kThreads), 0, stream, a);
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
 }
 
 }  // namespace
 
 int launch_paged_attention(const PagedAttnArgs& a, int head_dim, hipStream_t stream) {
   const bool e4m3 = a.c.elt == 1;
-  if (head_dim == 64)
-    e4m3 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
-  else
-    e4m3 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
-  const hipError_t err = hipGetLastError();
-  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
+  if (head_dim == 64) return e4m3 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
+  return e4m3 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
 }
 
 }  // namespace hk

@@ -91,10 +91,12 @@ class PagedKV:
     """One paged cache: ``pages`` pages of ``page_size`` slots for every layer, shared by up to ``seqs`` sequences of
     at most ``table_width`` pages.  All sequences are empty at first.
 
-    ``fork`` (and ``extend``, ``release``, ``truncate`` in its terms) changes which pages the sequences hold,
-    ``append`` stores new rows of the QKV projection, ``attention`` reads them, ``compact`` moves the live pages to
-    the front.  Activations are device buffers of bf16 rows; ``first`` is the list of the entries' first rows, one
-    longer than ``seqs``.  Calls are serialised by the caller.
+    ``fork`` (and ``extend``, ``release`` in its terms) changes which pages the sequences hold, ``append`` stores new
+    rows of the QKV projection, ``attention`` reads them, ``compact`` moves the live pages to the front.  Activations
+    are device buffers of bf16 rows; ``first`` is the list of the entries' first rows, one longer than ``seqs``.
+
+    A call waits for the one before (whatever its stream) before it hands its host arrays over: for one thread, and
+    not for capture into a graph, which is for the calls of ``lib()`` with arrays on the device.
     """
 
     def __init__(self, *, layers, kv_heads, head_dim, page_size, pages, seqs, table_width, dtype=BF16, k_scale=None,
@@ -123,15 +125,17 @@ class PagedKV:
                 raise ValueError(f"{name} must be [layers, kv_heads], finite and positive")
             self.bufs[name] = hip.DeviceBuffer.from_array(scale)
         hip.check(self._lib.hk_stream_sync(None), "sync")  # (the calls may go to other streams)
+        self._stream = None
         ptr = {name: b.ptr for name, b in self.bufs.items() if name not in ("workspace", "args")}
         self.cache = PagedCache(layer_stride=pages * page, page_stride=page, layers=layers, kv_heads=kv_heads,
                                 head_dim=head_dim, page_size=page_size, pages=pages, seqs=seqs,
                                 table_width=table_width, dtype=dtype, **ptr)
 
     def _args(self, stream, *arrays):
-        """Device copies of the calls' host arrays (None stays None), one behind the other.  The calls before have
-        read theirs when the stream is idle."""
-        hip.check(self._lib.hk_stream_sync(stream), "sync")
+        """Device copies of a call's host arrays (None stays None), one behind the other.  The call before has read
+        its own, and is through with the workspace, when its stream is idle."""
+        hip.check(self._lib.hk_stream_sync(self._stream), "sync")
+        self._stream = stream
         given = [a for a in arrays if a is not None]
         if sum(a.nbytes for a in given) > self.bufs["args"].nbytes:
             raise ValueError("more entries than the cache has sequences")
@@ -148,6 +152,8 @@ class PagedKV:
         once; waits for the outcome.  ValueError for an entry that is not valid, RuntimeError when the pages do not
         suffice; nothing is changed then."""
         n = len(child)
+        if n == 0:
+            return
         arrays = [_i32s(a, n, name) for a, name in ((child, "child"), (parent, "parent"), (keep, "keep"),
                                                     (grow, "grow"))]
         args = self._args(stream, *arrays)
@@ -179,7 +185,10 @@ class PagedKV:
         ``rope``: (cos, sin, positions) device tables, ``q_out`` (device pointer) receives the turned queries."""
         n, c = len(seqs), self.cache
         first = _i32s(first, n + 1, "first")
-        args = self._args(stream, _i32s(seqs, n, "seqs"), first)
+        seqs = _i32s(seqs, n, "seqs")
+        if len(np.unique(seqs)) < n:
+            raise ValueError("a sequence is listed twice")
+        args = self._args(stream, seqs, first)
         cos, sin, positions = rope or (None, None, 0)
         width = (q_heads + 2 * c.kv_heads) * c.head_dim
         hip.check(self._lib.hk_paged_append(ctypes.byref(c), layer, qkv, width, cos, sin, positions, *args, n,
@@ -199,6 +208,7 @@ class PagedKV:
 
     def compact(self, stream=None):
         """Moves the live pages to the front of the pool, in place; returns their number."""
+        self._args(stream)
         live = self.bufs["args"].ptr + self.bufs["args"].nbytes - 8
         hip.check(self._lib.hk_paged_compact(ctypes.byref(self.cache), self.cache.table, self.cache.refs, live,
                                              self.bufs["workspace"].ptr, stream), "hk_paged_compact")
@@ -206,7 +216,7 @@ class PagedKV:
         return int(self.bufs["args"].read(np.int32, 1, self.bufs["args"].nbytes - 8)[0])
 
     def _read(self, name, stream):
-        hip.check(self._lib.hk_stream_sync(stream), "sync")
+        self._args(stream)
         return self.bufs[name].read(np.int32, self.bufs[name].nbytes // 4)
 
     def lengths(self, stream=None):

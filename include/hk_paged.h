@@ -84,7 +84,8 @@ typedef struct hk_paged_cache {
  * head_dim / 2] float32 with positions >= table_width * page_size, or both
  * NULL for no rotation.  Tokens at negative positions (more rows than length)
  * are dropped, and their queries left as they were.  A sequence is listed
- * once.  Pointers and strides are multiples of 16 bytes. */
+ * once.  Fewer than 2^24 tokens.  Pointers and strides are multiples of 16
+ * bytes. */
 int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* qkv, int64_t qkv_stride,
                     const float* rope_cos, const float* rope_sin, int32_t positions, const int32_t* seqs,
                     const int32_t* first, int32_t n, int32_t tokens, int32_t q_heads, uint16_t* q_out,
@@ -98,10 +99,10 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
  * ln sum_j exp(scale q . k_j), by which results over parts of a context are
  * joined.  A row that sees nothing gets zeros and -inf.  Slots that a row does
  * not see have no influence on it, whatever they hold.  scale is finite and
- * positive.  max_new: the largest count of rows of one entry, as far as the
+ * positive.  out may be q itself, if the strides are equal.  max_new: the largest count of rows of one entry, as far as the
  * caller knows it; it chooses between forms of the kernel and every value
- * gives the same result, up to float32 summation order.
- * Pointers and strides are multiples of 16 bytes. */
+ * gives the same result, up to float32 summation order.  At most 2^30 rows
+ * (tokens x q_heads).  Pointers and strides are multiples of 16 bytes. */
 int hk_paged_attention(const hk_paged_cache* cache, int32_t layer, const uint16_t* q, int64_t q_stride,
                        const int32_t* seqs, const int32_t* first, int32_t n, int32_t tokens, int32_t max_new,
                        int32_t q_heads, float scale, int32_t window, uint16_t* out, int64_t out_stride, float* lse,

@@ -382,6 +382,60 @@ def test_attention_of_many_entries(hk_lib, n, counts):
     check_attention(*(x[rows] for x in got), tuple(w[rows] for w in want), _floats(q)[rows], cache, 0.125)
 
 
+@pytest.mark.parametrize("heads,kv_heads,rows", [(4096, 1, 1), (4096, 1024, 1), (1024, 1024, 3), (96, 1, 2)])
+def test_attention_of_many_heads(hk_lib, heads, kv_heads, rows):
+    announce(f"paged attention: {heads} heads on {kv_heads}")
+    rng = np.random.default_rng(heads + kv_heads)
+    cache = Cache(rng, pages=12, kv_heads=kv_heads, page=16, dim=64, seqs=2, width=6)
+    cache.give([70, 33], rng)
+    cache.fill(rng)
+    cache.upload()
+    first = [0, rows, 2 * rows]
+    q = _bits(rng.normal(size=(2 * rows, heads, 64)))
+    got = attention(cache, 0, q, [1, 0], first, scale=0.125)
+    check_attention(*got, oracle.attention(cache.o, 0, _floats(q), [1, 0], first, 0.125), _floats(q), cache, 0.125)
+
+
+@pytest.mark.parametrize("e4m3,counts", [(True, (1, 3)), (True, (90, 40)), (False, (1, 1))])
+def test_attention_with_the_smallest_scale(hk_lib, e4m3, counts):
+    """A scale whose product with k_scale underflows: the mean of the values that a row sees, and of no others."""
+    announce(f"paged attention: smallest scale, e4m3 {e4m3}, rows {counts}")
+    rng = np.random.default_rng(12)
+    cache = Cache(rng, pages=20, kv_heads=1, page=16, dim=64, seqs=2, width=10, e4m3=e4m3)
+    cache.give([150, 77], rng)
+    cache.fill(rng)
+    cache.upload()
+    first = np.cumsum([0] + list(counts))
+    q = _bits(rng.normal(size=(first[-1], 3, 64)))
+    got = attention(cache, 0, q, [0, 1], first, scale=1e-45, window=70)
+    check_attention(*got, oracle.attention(cache.o, 0, _floats(q), [0, 1], first, 1e-45, 70), _floats(q), cache, 1e-45)
+
+
+@pytest.mark.parametrize("dim,e4m3,counts,lengths", [
+    (64, False, (1, 1, 1), (4000, 30, 1)), (128, False, (200, 1, 60), (2000, 300, 61)), (128, True, (120,), (3500,)),
+    (64, False, (40, 3, 0), (900, 2500, 5))])
+def test_attention_in_place(hk_lib, dim, e4m3, counts, lengths):
+    """The results in the queries' memory, of whole and of split tasks: the same bits as beside them."""
+    from runtime import hip, paged
+
+    announce(f"paged attention: in place, dim {dim}, {counts}")
+    rng = np.random.default_rng(61)
+    need = sum(-(-n // 16) for n in lengths)
+    cache = Cache(rng, pages=need, kv_heads=2, page=16, dim=dim, seqs=len(counts), width=need, e4m3=e4m3)
+    cache.give(list(lengths), rng)
+    cache.fill(rng)
+    cache.upload()
+    first = np.cumsum([0] + list(counts))
+    q = _bits(rng.normal(size=(first[-1], 8, dim)))
+    want = attention(cache, 0, q, range(len(counts)), first, scale=0.1)[2]
+    Q, F = _dev(q), _dev(first.astype(np.int32))
+    hip.check(paged.lib().hk_paged_attention(
+        ctypes.byref(cache.c), 0, Q.ptr, 8 * dim, None, F.ptr, len(counts), first[-1], max(counts), 8, 0.1, 0, Q.ptr,
+        8 * dim, None, cache.bufs["workspace"].ptr, None), "hk_paged_attention")
+    _sync()
+    np.testing.assert_array_equal(Q.read(np.uint16, q.size).reshape(q.shape), want)
+
+
 def test_attention_on_two_streams(hk_lib):
     """Calls in flight at once on streams of their own, each with its workspace; then the same stream after stream."""
     from runtime import hip, paged
@@ -825,12 +879,19 @@ def test_chats_share_a_prompt(hk_lib):
             kv.attention(layer, Q.ptr, seqs, first, hq, OUT.ptr)
             _sync()
             oracle.append(o, layer, _floats(x), seqs, first, hq, cos, sin, lambda rows, which: _floats(_bits(rows)))
+            # The float32 rotation may fall to the neighbouring bf16, 2^-7 of the smaller one at most (and where the
+            # two products cancel, by 2^-22 of either): the attention is checked on what the pool holds.
+            for y in "kv":
+                pool = _floats(kv.bufs[y].read(np.uint16, kv.bufs[y].nbytes // 2).reshape(o[y].shape)[layer])
+                mine = np.any(o[y][layer] != 0, axis=-1)  # slots that were written: the others hold anything
+                was, got = o[y][layer][mine], pool[mine]
+                assert np.all(np.abs(got - was) <= 2.0**-7 * np.abs(was) + 2.0**-20)
+                o[y][layer][mine] = got
             q = _floats(Q.read(np.uint16, Q.nbytes // 2).reshape(-1, hq, dim))
             got = _floats(OUT.read(np.uint16, OUT.nbytes // 2).reshape(-1, hq, dim))
             want, _, spread = oracle.attention(o, layer, q, seqs, first, dim**-0.5)
-            # the keys' float32 rotation may round to the neighbouring bf16: 2^-8 |k_d| at every dimension, so a score
-            # by up to 2^-8 scale sum |q_d k_d|, a few per cent of the keys; then the tolerances of the top
-            tol = 2.0**-8 * np.abs(want) + (2.0**-8 + 2.0**-8) * spread + 1e-30
+            e_s = dim * 2.0**-24 * np.linalg.norm(q, axis=-1) * np.abs(o["k"]).max() * 1.01 + 2.0**-23 * 64
+            tol = 2.0**-8 * (np.abs(want) + spread) + (2 * e_s[..., None] + 2.0**-18) * spread + 1e-30
             assert np.all(np.abs(got - want) <= tol)
 
     forked([0], [0], [0], [21])
@@ -859,4 +920,57 @@ def test_chats_share_a_prompt(hk_lib):
         kv.fork([0], [1], [5], [0])
     with pytest.raises(RuntimeError):
         kv.fork([0, 1, 2, 3], [0] * 4, [0] * 4, [8 * page] * 4)
+    with pytest.raises(ValueError):
+        kv.append(0, C.ptr, [1, 1], [0, 1, 2], hq)
+    with pytest.raises(ValueError):
+        kv.extend([5], [1])
+    with pytest.raises(ValueError):
+        kv.attention(0, C.ptr, [0, 1], [0, 1], hq, S.ptr)
+    kv.fork([], [], [], [])
+    assert np.all(kv.refs() == 0) and kv.compact() == 0
     kv.close()
+
+
+def test_cache_calls_from_stream_to_stream(hk_lib):
+    """PagedKV's calls on alternating streams, each with other sequences: none overtakes the arguments or the
+    workspace of the one before."""
+    from runtime import hip, paged
+
+    announce("paged cache: stream to stream")
+    rng = np.random.default_rng(71)
+    hq, hkv, dim, page = 4, 2, 64, 16
+    kv = paged.PagedKV(layers=1, kv_heads=hkv, head_dim=dim, page_size=page, pages=400, seqs=6, table_width=70)
+    lengths = [900, 20, 1000, 3, 700, 64]
+    streams = []
+    for _ in range(2):
+        handle = ctypes.c_void_p()
+        hip.check(hk_lib.hk_stream_create(ctypes.byref(handle)), "hk_stream_create")
+        streams.append(handle.value)
+    o = {"k": np.zeros((1, 400, hkv, page, dim)), "v": np.zeros((1, 400, hkv, page, dim)),
+         "table": np.full((6, 70), -1, np.int32), "length": np.zeros(6, np.int32), "refs": np.zeros(400, np.int32)}
+    first = np.cumsum([0] + lengths)
+    x = _bits(rng.normal(size=(first[-1], hq + 2 * hkv, dim)))
+    IN = _dev(x)
+    row = 2 * (hq + 2 * hkv) * dim
+    assert oracle.fork(o, range(6), range(6), [0] * 6, lengths) == (0, 0)
+    kv.extend(range(6), lengths, streams[0])
+    for s in range(6):  # a sequence a call, from stream to stream
+        kv.append(0, IN.ptr + int(first[s]) * row, [s], [0, lengths[s]], hq, stream=streams[s % 2])
+    oracle.append(o, 0, _floats(x), range(6), first, hq, None, None, lambda rows, which: rows)
+    batches = [[s] for s in range(6)] + [[5, 0], [2, 4, 1], [3, 0, 2]]
+    q = _bits(rng.normal(size=(len(batches), 3, hq, dim)))
+    Q, OUT, SIZE = _dev(q), _dev(np.zeros(q.shape, np.uint16)), 2 * 3 * hq * dim
+    for i, batch in enumerate(batches):
+        kv.attention(0, Q.ptr + i * SIZE, batch, np.arange(len(batch) + 1), hq, OUT.ptr + i * SIZE, stream=streams[i % 2])
+    for stream in streams:
+        hip.check(hk_lib.hk_stream_sync(stream), "sync")
+    got = _floats(OUT.read(np.uint16, q.size).reshape(q.shape))
+    for i, batch in enumerate(batches):
+        n = len(batch)
+        want, _, spread = oracle.attention(o, 0, _floats(q[i, :n]), batch, np.arange(n + 1), dim**-0.5)
+        # (a score's float32 error is below 64 2^-24 5^2 64 / 8 < 2^-10 for these draws)
+        tol = 2.0**-8 * (np.abs(want) + spread) + (2.0**-9 + 2.0**-18) * spread + 1e-30
+        assert np.all(np.abs(got[i, :n] - want) <= tol)
+    kv.close()
+    for stream in streams:
+        hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")

@@ -102,9 +102,11 @@ def test_refuses_bad_arguments():
         _refused("hk_paged_append", _cache(), bad, **changes)
     for changes in (dict(q=None), dict(out=None), dict(q=AT + 8), dict(out=AT + 4), dict(q_stride=248),
                     dict(out_stride=260), dict(workspace=None), dict(workspace=AT + 16), dict(max_new=0),
-                    dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                    dict(out=AT, out_stride=264), dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                     dict(scale=float("inf"))):
         _refused("hk_paged_attention", _cache(), bad, **changes)
+    _refused("hk_paged_append", _cache(), hip.HK_ERR_UNSUPPORTED, tokens=1 << 24)
+    _refused("hk_paged_attention", _cache(), hip.HK_ERR_UNSUPPORTED, tokens=(1 << 28) + 1)
     for changes in (dict(status=None), dict(workspace=None), dict(workspace=AT + 8), dict(n=0), dict(n=5)):
         _refused("hk_paged_fork", _cache(), bad, **changes)
     _refused("hk_paged_fork", _cache(seqs=30000, table_width=1000), hip.HK_ERR_UNSUPPORTED, n=30000)
