@@ -41,6 +41,7 @@ struct PagedAttnArgs {
   int q_heads, group, window, max_new;
   PlanDivisor by_group;    // set by the launch
   int rows_min, rows_max;  // set by the launch: rows (tokens x group) of the entries it takes
+  int ticket0, part0;      // set by the launch: its first ticket, and byte of partial results
   float scale;
   void* workspace;
 };

@@ -83,22 +83,42 @@ __device__ __forceinline__ Entry load_entry(const PagedAttnArgs& a, int b) {
   return {is ? s : -1, f0, {length, f1 - f0}};
 }
 
-// Whether an entry of `count` rows is this launch's (a batch of long and short
-// entries is two launches).
+// Whether an entry of `count` rows is this form's (a batch may have long and
+// short entries).
 __device__ __forceinline__ bool takes(const PagedAttnArgs& a, int count) {
   return count > 0 && count * a.group >= a.rows_min && count * a.group <= a.rows_max;
+}
+
+// v of another lane as the DPP control says; 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+// Sum of v over the lanes up to this one: within rows of 16, then the rows
+// before.  (With these and without barriers for up to 64 entries 16 chats' check
+// of five tokens takes 20.0 us; with __shfl_up through the LDS crossbar and the
+// workgroup's barriers it took 21.0.)
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+  v += dpp<0x111, 0xf>(v);  // row_shr:1
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast:15, to rows 1 and 3
+  v += dpp<0x143, 0xc>(v);  // row_bcast:31, to rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)lane_of((int)(v >> 32), lane) << 32 | (uint32_t)lane_of((int)v, lane));
 }
 
 // Sum of v over the workgroup in every thread, and the sum of the threads
 // before this one.
 __device__ __forceinline__ int64_t scan(int64_t v, int64_t* sums, int64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t s = v;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int64_t u = __shfl_up(s, m, 64);
-    if (lane >= m) s += u;
-  }
+  const int64_t s = wave_scan(v);
   __syncthreads();
   if (lane == 63) sums[wave] = s;
   __syncthreads();
@@ -122,9 +142,7 @@ __device__ __forceinline__ int64_t wave_head_units(const PlanShape& s, const Pla
   int64_t n = 0;
   const int tiles = plan_tiles(s, e);
   for (int t = threadIdx.x & 63; t < tiles; t += 64) n += plan_units(s, plan_span(s, e, t));
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m, 64);
-  return uniform(n);
+  return lane_of(wave_scan(n), 63);
 }
 __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
   const int lane = threadIdx.x & 63, tiles = plan_tiles(s, e);
@@ -136,22 +154,17 @@ __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEnt
   if (tiles == 1) return p;
   for (;; p.tile += 64) {
     const int64_t u = wave_units(s, e, p.tile + lane);
-    int64_t sum = u;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int64_t v = __shfl_up(sum, m, 64);
-      if (lane >= m) sum += v;
-    }
+    const int64_t sum = wave_scan(u);
     const unsigned long long past = __ballot(sum > rem);
     if (past == 0 && p.tile + 64 < tiles) {
-      const int64_t all = uniform(__shfl(sum, 63, 64));
+      const int64_t all = lane_of(sum, 63);
       rem -= all;
       p.start += all;
       continue;
     }
     const int at = past ? __builtin_ctzll(past) : 63;
     p.tile += at;
-    p.start += uniform(__shfl(sum - u, at, 64));
+    p.start += lane_of(sum - u, at);
     return p;
   }
 }
@@ -214,11 +227,20 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
     // entries of more tiles: the wave's lanes together
     for (unsigned long long todo = __ballot(has && !few); todo; todo &= todo - 1) {
       const int l = __builtin_ctzll(todo);
-      const int64_t v = wave_head_units(s, {uniform(__shfl(e.length, l, 64)), uniform(__shfl(e.count, l, 64))});
+      const int64_t v = wave_head_units(s, {lane_of(e.length, l), lane_of(e.count, l)});
       if ((int)(threadIdx.x & 63) == l) u = s.heads * v;
     }
     return u;
   };
+  if (n <= 64) {  // each wave knows all entries: no barrier
+    const int64_t mine = units(threadIdx.x & 63), sum = wave_scan(mine);
+    if (!cut(lane_of(sum, 63))) return false;
+    const int64_t before = sum - mine;
+    const int l = __builtin_ctzll(__ballot(before <= run.begin && run.begin < sum));
+    run.entry = {lane_of(seq.x, l), lane_of(rows.x, l), {lane_of(seq.y, l), lane_of(rows.y - rows.x, l)}};
+    run.place = wave_find(s, run.entry.e, l, lane_of(before, l), run.begin - lane_of(before, l));
+    return true;
+  }
   // (up to as many entries as threads, the units are worked out once)
   int64_t mine = units(threadIdx.x), total, before = scan(mine, sums, total);
   if (n > kThreads) {
@@ -375,7 +397,7 @@ struct Pending {
 // write-back as a fence would do).  The joining workgroup leaves the ticket at
 // zero.
 __device__ __forceinline__ int draw_tickets(const PagedAttnArgs& a, const Pending (&pend)[2], int n, int* last) {
-  unsigned* const tickets = static_cast<unsigned*>(a.workspace);
+  unsigned* const tickets = static_cast<unsigned*>(a.workspace) + a.ticket0;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if ((int)threadIdx.x < n) {
@@ -392,7 +414,8 @@ __device__ __forceinline__ int draw_tickets(const PagedAttnArgs& a, const Pendin
 
 // The partial results as one buffer; byte offset of workgroup w's part.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_of(const PagedAttnArgs& a) {
-  return rsrc(static_cast<char*>(a.workspace) + 4 * kPagedTicketWords, HK_PAGED_WORKSPACE - 4 * kPagedTicketWords);
+  const int at = 4 * kPagedTicketWords + a.part0;
+  return rsrc(static_cast<char*>(a.workspace) + at, HK_PAGED_WORKSPACE - at);
 }
 
 // The rows [r0, r0 + rows) of kv head g once more, a wave per row, 64 slots at a
@@ -463,7 +486,8 @@ struct Narrow {
   static constexpr int kVLoads = kRowBytes / 64;           // per 16 slots
   static constexpr int kDims = D / 16;
   static constexpr int kPitch = D + 4;                     // floats of a row of O in LDS
-  static constexpr int kLds = kNarrowSlots * D * 2 > 16 * kPitch * 4 ? kNarrowSlots * D * 2 : 16 * kPitch * 4;
+  static constexpr int kLds = kNarrowSlots * D * 2 > 16 * kPitch * 4 ? kNarrowSlots * D * 2 : 16 * kPitch * 4;  // of a wave
+  static constexpr int kSmem = kWaves * kLds;
   // floats of a task's partial result: O [rows][D], max [rows], sum [rows]
   static constexpr int kPart = kRows * (D + 2);
 };
@@ -480,9 +504,9 @@ __device__ __forceinline__ int v_key(int r) {
 constexpr int narrow_per_cu(int d, bool e4m3, int nq) { return nq == 2 ? 2 : d == 64 ? 4 : e4m3 ? 3 : 2; }
 
 template <int D, bool E4M3, int NQ>
-__global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_narrow_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ void narrow_tasks(const PagedAttnArgs& a, char* smem) {
   using N = Narrow<D, E4M3, NQ>;
-  __shared__ __attribute__((aligned(16))) char lds[kWaves][N::kLds];
+  char (&lds)[kWaves][N::kLds] = *reinterpret_cast<char (*)[kWaves][N::kLds]>(smem);
   __shared__ float wm[kWaves][N::kRows], wl[kWaves][N::kRows];
   __shared__ int last[2], again[kWaves];
   constexpr int kJoin = D * NQ == 256 ? 8 : 16;  // parts at a time
@@ -887,6 +911,7 @@ template <int D>
 struct Wide {
   static constexpr int kRows = 128;
   static constexpr int kBuf = kWideSlots * D;  // bf16 of one of K, V
+  static constexpr int kSmem = 4 * kBuf * 2;
   // floats of a part: O, max and sum per lane
   static constexpr int kLaneFloats = D / 2 + 2;
   static constexpr int kPart = kThreads * kLaneFloats;
@@ -918,11 +943,11 @@ template <int N>
 using At = std::integral_constant<int, N>;
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ void wide_tasks(const PagedAttnArgs& a, char* smem) {
   using W = Wide<D>;
   constexpr int kRowBytes = D * (E4M3 ? 1 : 2), kLoads = kRowBytes / 64, kSteps = D / 16, kDims = D / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[2][W::kBuf];
-  __shared__ __attribute__((aligned(16))) uint16_t vs_lds[2][W::kBuf];
+  uint16_t (&ks_lds)[2][W::kBuf] = *reinterpret_cast<uint16_t (*)[2][W::kBuf]>(smem);
+  uint16_t (&vs_lds)[2][W::kBuf] = *reinterpret_cast<uint16_t (*)[2][W::kBuf]>(smem + W::kSmem / 2);
   // of each 16 slots of a block: bit 0: they have a page, bit 1: an infinity or
   // NaN among the values, where not every row sees them all
   __shared__ __attribute__((aligned(16))) int note_lds[2][kWaves];
@@ -1269,22 +1294,32 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    for (int k = 0; has && k < pp.count; ++k) {
-      const int slot = plan_slot(pp, pp.first + k) * (W::kPart * 4);
-      const u32x2_t ml = __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * kQuads + 8 * tid, 0, kSc1);
-      u32x4 y[kQuads];
+    // two parts go out at once (a 2039-token piece: 1088 us, one at a time 1103)
+    for (int k0 = 0; has && k0 < pp.count; k0 += 2) {
+      u32x2_t ml[2];
+      u32x4 y[2][kQuads];
 #pragma unroll
-      for (int i = 0; i < kQuads; ++i)
-        y[i] = __builtin_amdgcn_raw_buffer_load_b128(parts, slot + 16 * (kThreads * i + tid), 0, kSc1);
-      const float mk = __uint_as_float(ml.x), m_new = fmaxf(m, mk);
-      const float f0 = __builtin_amdgcn_exp2f(m - finite_max(m_new)), f1 = __builtin_amdgcn_exp2f(mk - finite_max(m_new));
-      note |= mk != mk;
-      l = l * f0 + __uint_as_float(ml.y) * f1;
-      m = m_new;
+      for (int j = 0; j < 2; ++j) {
+        const int slot = plan_slot(pp, pp.first + min(k0 + j, pp.count - 1)) * (W::kPart * 4);
+        ml[j] = __builtin_amdgcn_raw_buffer_load_b64(parts, slot + 16 * kThreads * kQuads + 8 * tid, 0, kSc1);
 #pragma unroll
-      for (int i = 0; i < kQuads; ++i)
+        for (int i = 0; i < kQuads; ++i)
+          y[j][i] = __builtin_amdgcn_raw_buffer_load_b128(parts, slot + 16 * (kThreads * i + tid), 0, kSc1);
+      }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[i][c]), f1, o[i / 4][4 * (i % 4) + c] * f0);
+      for (int j = 0; j < 2; ++j) {
+        if (k0 + j >= pp.count) break;
+        const float mk = __uint_as_float(ml[j].x), m_new = fmaxf(m, mk);
+        const float f0 = __builtin_amdgcn_exp2f(m - finite_max(m_new)), f1 = __builtin_amdgcn_exp2f(mk - finite_max(m_new));
+        note |= mk != mk;
+        l = l * f0 + __uint_as_float(ml[j].y) * f1;
+        m = m_new;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            o[i / 4][4 * (i % 4) + c] = fmaf(__uint_as_float(y[j][i][c]), f1, o[i / 4][4 * (i % 4) + c] * f0);
+      }
     }
     const int any = __any(note);
     if (lane == 0) again[wave] = any;
@@ -1297,16 +1332,61 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
   }
 }
 
-// Launches: as many workgroups as the GPU holds at once.
-constexpr int kCus = 256;
-constexpr bool fits(long long groups, long long part) {
-  return groups <= kPagedTicketWords && groups % 8 == 0 &&
-         4ll * kPagedTicketWords + 2 * groups * part * 4 <= HK_PAGED_WORKSPACE;
+// ---- kernels ----
+
+template <int D, bool E4M3, int NQ>
+__global__ __launch_bounds__(kThreads, narrow_per_cu(D, E4M3, NQ)) void paged_narrow_kernel(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[Narrow<D, E4M3, NQ>::kSmem];
+  narrow_tasks<D, E4M3, NQ>(a, smem);
 }
-static_assert(fits(4 * kCus, Narrow<64, false, 1>::kPart) && fits(3 * kCus, Narrow<128, true, 1>::kPart) &&
-                  fits(2 * kCus, Narrow<128, false, 2>::kPart) && fits(kCus * wide_per_cu(128), Wide<128>::kPart) &&
-                  fits(kCus * wide_per_cu(64), Wide<64>::kPart),
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[Wide<D>::kSmem];
+  wide_tasks<D, E4M3>(a, smem);
+}
+
+// Entries of a few rows (few) beside longer ones (many), each in its form: a
+// workgroup takes its run of the ones, then its run of the others, without
+// waiting for the workgroups that are behind.  Pieces of prompts beside chats
+// with a window: 58.6 us, in two launches 65.0; 20 sequences of up to 9000
+// slots, 7 of them with 511 new tokens, head_dim 128: 287 and 301.  (Workgroups
+// that begin with the others, so that reading and products go on at the same
+// time, gain no more: 60.0 and 289.)
+constexpr int kCus = 256;
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_mixed_kernel(PagedAttnArgs few, PagedAttnArgs many) {
+  constexpr int kSmem = Narrow<D, E4M3, 1>::kSmem > Wide<D>::kSmem ? Narrow<D, E4M3, 1>::kSmem : Wide<D>::kSmem;
+  __shared__ __attribute__((aligned(16))) char smem[kSmem];
+  narrow_tasks<D, E4M3, 1>(few, smem);
+  __syncthreads();
+  wide_tasks<D, E4M3>(many, smem);
+}
+
+// Launches: as many workgroups as the GPU holds at once.
+constexpr int64_t part_bytes(long long groups, long long part) { return 2 * groups * part * 4; }
+constexpr bool fits(long long groups, long long bytes) {
+  return groups <= kPagedTicketWords && groups % 8 == 0 && 4ll * kPagedTicketWords + bytes <= HK_PAGED_WORKSPACE;
+}
+template <int D, bool E4M3, int NQ>
+constexpr bool narrow_fits() {
+  constexpr int groups = kCus * narrow_per_cu(D, E4M3, NQ);
+  return fits(groups, part_bytes(groups, Narrow<D, E4M3, NQ>::kPart));
+}
+template <int D>
+constexpr bool wide_fits() {  // with the narrow form's beside it
+  constexpr int groups = kCus * wide_per_cu(D);
+  return fits(2 * groups, part_bytes(groups, Wide<D>::kPart) + part_bytes(groups, Narrow<D, false, 1>::kPart));
+}
+static_assert(narrow_fits<64, false, 1>() && narrow_fits<64, true, 1>() && narrow_fits<128, false, 1>() &&
+                  narrow_fits<128, true, 1>() && narrow_fits<64, false, 2>() && narrow_fits<64, true, 2>() &&
+                  narrow_fits<128, false, 2>() && narrow_fits<128, true, 2>() && wide_fits<64>() && wide_fits<128>(),
               "partial results and tickets fit the workspace");
+
+int launched() {
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
+}
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
 // most as far as the caller knows.
@@ -1316,28 +1396,34 @@ int narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kCus * narrow_per_cu(D, E4M3, 1)), dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kCus * narrow_per_cu(D, E4M3, 2)), dim3(kThreads), 0, stream, a);
-  const hipError_t err = hipGetLastError();
-  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
+  return launched();
 }
 
 template <int D, bool E4M3>
 int launch(PagedAttnArgs a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_new * a.group;
+  const dim3 wide_groups(kCus * wide_per_cu(D));
   a.by_group = plan_divisor(a.group);
   a.rows_min = 1;
   a.rows_max = INT32_MAX;
+  a.ticket0 = a.part0 = 0;
   if (rows <= 64) return narrow<D, E4M3>(a, rows, stream);
-  // entries of a few rows beside longer ones: a launch of their own
+  // entries of a few rows beside longer ones
   const int few = a.group <= 16 ? 16 : 32;
   if (a.b.n > 1 && a.group <= few) {
     PagedAttnArgs b = a;
     b.rows_max = few;
     a.rows_min = few + 1;
+    if (few == 16) {
+      a.ticket0 = wide_groups.x;
+      a.part0 = (int)part_bytes(wide_groups.x, Narrow<D, E4M3, 1>::kPart);
+      hipLaunchKernelGGL((paged_mixed_kernel<D, E4M3>), wide_groups, dim3(kThreads), 0, stream, b, a);
+      return launched();
+    }
     if (const int rc = narrow<D, E4M3>(b, few, stream)) return rc;
   }
-  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3>), dim3(kCus * wide_per_cu(D)), dim3(kThreads), 0, stream, a);
-  const hipError_t err = hipGetLastError();
-  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
+  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3>), wide_groups, dim3(kThreads), 0, stream, a);
+  return launched();
 }
 
 }  // namespace
