@@ -8,6 +8,7 @@ directory's parent on ``sys.path`` and import ``runtime.generate`` /
 - ``runtime.qwen_engine``  ``QwenDecoderEngine``: every layer + head per step
 - ``runtime.engine``       ``DecoderEngine``: layers + final norm (SmolLM form)
 - ``runtime.generate``     ``NPUDecoder``: the step API used by servers and chat
+- ``runtime.paged``        ``PagedKV``: a paged KV cache of many sequences
 - ``runtime.synthetic``    seeded random-init models of the benchmark shapes
 - ``runtime.bf16``         host-side bfloat16 bit conversions
 """
