@@ -135,7 +135,8 @@ c = ctypes.byref(paged.PagedCache(k=at, v=at, table=at, length=at, refs=at, laye
 calls = {
     "append": lambda: lib.hk_paged_append(c, 1, at, 512, at, at, 64, None, at, 2, 3, 4, at + 1024, 256, stream),
     "token": lambda: lib.hk_paged_attention(c, 1, at, 256, None, at, 2, 3, 1, 4, 0.125, 0, at, 256, None, at, stream),
-    "pieces": lambda: lib.hk_paged_attention(c, 1, at, 256, None, at, 2, 300, 99, 4, 0.125, 0, at, 256, None, at, stream),
+    "mixed": lambda: lib.hk_paged_attention(c, 1, at, 256, None, at, 2, 300, 99, 4, 0.125, 0, at, 256, None, at, stream),
+    "pieces": lambda: lib.hk_paged_attention(c, 1, at, 4096, None, at, 2, 300, 99, 64, 0.125, 0, at, 4096, None, at, stream),
     "fork": lambda: lib.hk_paged_fork(c, None, None, None, None, 2, at, at, stream),
     "compact": lambda: lib.hk_paged_compact(c, at, at, at, at, stream),
 }
