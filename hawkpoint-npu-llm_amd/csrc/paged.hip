@@ -599,6 +599,9 @@ MoveArgs moves_of(const hk_paged_cache* c, const Move* moves, const int* count, 
   return m;
 }
 
+// Eight workgroups per CU: 16 KiB in flight each.  Four take 15.7 us instead of
+// 14.9 for the 512-page pool and 136 instead of 133 for 192 answers, sixteen
+// 13.4 instead of 12.8 for a step that copies nothing.
 constexpr int kMoveGroups = 2048;
 
 int launched(const char* what) {

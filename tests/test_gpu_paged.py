@@ -197,6 +197,8 @@ CASES = [
     ("a piece of a prompt, e4m3", 4, 2, 128, 16, True, [(515, 150)], 0),
     ("a piece of a prompt, e4m3, 64 wide", 6, 2, 64, 16, True, [(515, 150)], 0),
     ("pieces beside tokens", 8, 2, 64, 16, False, [(300, 100), (50, 1), (129, 1), (64, 64), (700, 1)], 0),
+    ("pieces beside tokens, 24 heads per kv head", 48, 2, 64, 16, False, [(300, 40), (50, 1), (129, 1), (64, 2), (700, 1)], 0),
+    ("the same, 20 heads, 128 wide, a window", 20, 1, 128, 32, True, [(300, 40), (50, 1), (129, 3), (700, 1), (9, 9)], 90),
     ("pieces beside tokens, 128 wide", 6, 2, 128, 64, True, [(300, 100), (50, 1), (129, 1), (64, 64), (700, 1)], 0),
     ("window of one", 4, 2, 64, 16, False, [(100, 1), (30, 30)], 1),
     ("window inside a tile", 4, 2, 64, 16, False, [(100, 1), (300, 90), (20, 20)], 37),
@@ -761,6 +763,63 @@ def test_fork_and_compact_sizes(hk_lib, pages, seqs):
     np.testing.assert_array_equal(R.read(np.int32, pages), cache.o["refs"])
     cache.o.update(was)
     same(cache)
+
+
+def test_far_pages_are_written_copied_and_moved(hk_lib):
+    """Pages 2 GiB apart: an append, a fork that copies slots and a compaction that moves pages more than 4 GiB away."""
+    from runtime import hip, paged
+
+    announce("paged cache: writes beyond 32-bit offsets")
+    rng = np.random.default_rng(9)
+    cache = Cache(rng, pages=6, kv_heads=1, page=16, dim=64, seqs=3, width=5, poison=False)
+    cache.o["table"][0, 0], cache.o["table"][2, :4] = 5, [0, 1, 2, 3]
+    cache.o["refs"][:] = (1, 1, 1, 1, 0, 1)
+    cache.o["length"][:] = (10, 0, 60)
+    cache.fill(rng)
+    cache.upload()
+    stride, size = 1 << 30, 16 * 64
+    far = {x: hip.DeviceBuffer(2 * (5 * stride + size)) for x in "kv"}
+
+    def put():
+        for x in "kv":
+            for p in range(6):
+                far[x].write(cache.encode(cache.o[x][0], x, 0)[p], 2 * p * stride)
+
+    def held():
+        for x in "kv":
+            want = cache.encode(cache.o[x][0], x, 0)
+            for s in range(3):
+                for j in range(int(cache.o["length"][s])):
+                    p = int(cache.o["table"][s, j // 16])
+                    got = far[x].read(np.uint16, size, 2 * p * stride).reshape(1, 16, 64)
+                    np.testing.assert_array_equal(got[:, j % 16], want[p, :, j % 16])
+
+    put()
+    for x in "kv":
+        setattr(cache.c, x, far[x].ptr)
+    cache.c.page_stride = cache.c.layer_stride = stride
+    step = ([0, 1], [0, 0], [10, 10], [1, 2])
+    assert fork(cache, *step) == oracle.fork(cache.o, *step) == (0, 0)  # sequence 1 gets page 4
+    assert cache.o["table"][1, 0] == 4
+    held()
+    x = _bits(rng.normal(size=(3, 4, 64)))
+    IN, SEQS, FIRST = _dev(x), _dev(np.array([0, 1], np.int32)), _dev(np.array([0, 1, 3], np.int32))
+    hip.check(paged.lib().hk_paged_append(ctypes.byref(cache.c), 0, IN.ptr, 256, None, None, 0, SEQS.ptr, FIRST.ptr, 2, 3, 2,
+                                          None, 0, None), "hk_paged_append")
+    _sync()
+    oracle.append(cache.o, 0, _floats(x), [0, 1], [0, 1, 3], 2, None, None, lambda rows, which: rows)
+    held()
+    free = ([2], [2], [0], [0])
+    assert fork(cache, *free) == oracle.fork(cache.o, *free) == (0, 0)
+    LIVE = _dev(np.zeros(1, np.int32))
+    hip.check(paged.lib().hk_paged_compact(ctypes.byref(cache.c), cache.c.table, cache.c.refs, LIVE.ptr,
+                                           cache.bufs["workspace"].ptr, None), "hk_paged_compact")
+    _sync()
+    assert LIVE.read(np.int32, 1)[0] == oracle.compact(cache.o) == 2
+    assert sorted(cache.o["table"][:2, 0]) == [0, 1]
+    for name in ("table", "length", "refs"):
+        np.testing.assert_array_equal(cache.bufs[name].read(np.int32, cache.o[name].size), cache.o[name].ravel())
+    held()
 
 
 # ---- together ----
