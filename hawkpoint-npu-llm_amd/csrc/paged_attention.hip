@@ -484,7 +484,8 @@ __device__ __forceinline__ void rows_again(const PagedAttnArgs& a, const Entry& 
 // us, the workgroups' unequal ends 5 to 10, tickets and joins 7.  190 chats in
 // e4m3 (270 MB): 62 us, 38 at that rate.  16 chats' check of five tokens (35
 // rows, 15 MB): 20 us, of these 3 to plan, 4 in the loop, 8 to join some twenty
-// parts of a task.  One chat of 71 slots: 6.4 us, a launch alone 3.8.
+// parts of a task (its two tiles as one of 64 rows: 24.5 us).  One chat of 71
+// slots: 6.4 us, a launch alone 3.8.
 constexpr int kNarrowSlots = 32;
 
 template <int D, bool E4M3, int NQ>
