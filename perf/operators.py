@@ -16,7 +16,6 @@ table entries that name page p.  Kinds of case:
 """
 
 import ctypes
-import functools
 import math
 import random
 import sys
@@ -273,7 +272,6 @@ def prepare(case, seed):
 # ---- the framework's calls ----
 
 
-@functools.lru_cache(None)  # (a program imports once, not with every call)
 def _package():
     here = str(Path(__file__).resolve().parents[1] / "hawkpoint-npu-llm_amd")
     if here not in sys.path:
