@@ -5,6 +5,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
+#include "hk_internal.h"
 #include "hk_paged.h"
 #include "paged_plan.h"
 
@@ -48,6 +51,21 @@ struct PagedAttnArgs {
 int launch_paged_attention(const PagedAttnArgs& a, int head_dim, hipStream_t stream);
 
 #ifdef __HIPCC__
+// A launch, and its own error: hipGetLastError would also give one that an
+// earlier HIP call of the caller's has left, and a fork that stopped for that
+// between its two launches would leave pages that nobody has copied.
+template <typename... P, typename... A>
+int paged_launch(const char* what, void (*kernel)(P...), int groups, int threads, hipStream_t stream, const A&... args) {
+  std::tuple<P...> given(args...);
+  const hipError_t err = std::apply(
+      [&](auto&... a) {
+        void* at[] = {&a...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(groups), dim3(threads), at, 0, stream);
+      },
+      given);
+  return err == hipSuccess ? 0 : hip_fail(err, what);
+}
+
 // Rows of entry b, within the batch's rows whatever `first` holds.
 __device__ __forceinline__ int2 entry_rows(const PagedBatch& b, int entry) {
   const int f0 = min(max(b.first[entry], 0), b.tokens);

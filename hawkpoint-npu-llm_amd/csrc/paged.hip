@@ -604,11 +604,6 @@ MoveArgs moves_of(const hk_paged_cache* c, const Move* moves, const int* count, 
 // 13.4 instead of 12.8 for a step that copies nothing.
 constexpr int kMoveGroups = 2048;
 
-int launched(const char* what) {
-  const hipError_t err = hipGetLastError();
-  return err == hipSuccess ? 0 : hip_fail(err, what);
-}
-
 #define HK_TRY(call)            \
   do {                          \
     const int rc_ = (call);     \
@@ -648,16 +643,9 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
                   q_out_stride, q_heads};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool e4m3 = cache->dtype == HK_PAGED_E4M3;
-  const dim3 grid(tokens), block(256);
-  if (d == 64 && !e4m3)
-    hipLaunchKernelGGL((paged_append_kernel<64, false>), grid, block, 0, st, a);
-  else if (d == 64)
-    hipLaunchKernelGGL((paged_append_kernel<64, true>), grid, block, 0, st, a);
-  else if (!e4m3)
-    hipLaunchKernelGGL((paged_append_kernel<128, false>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((paged_append_kernel<128, true>), grid, block, 0, st, a);
-  return launched("paged append launch");
+  const auto kernel = d == 64 ? (e4m3 ? paged_append_kernel<64, true> : paged_append_kernel<64, false>)
+                              : (e4m3 ? paged_append_kernel<128, true> : paged_append_kernel<128, false>);
+  return paged_launch("paged append launch", kernel, tokens, 256, st, a);
 }
 
 int hk_paged_attention(const hk_paged_cache* cache, int32_t layer, const uint16_t* q, int64_t q_stride,
@@ -734,13 +722,9 @@ int hk_paged_fork(const hk_paged_cache* cache, const int32_t* child, const int32
   a.rows = a.fresh + a.pages;
   a.moves = reinterpret_cast<Move*>(a.rows + (int64_t)n * a.width);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n <= kForkLds)
-    hipLaunchKernelGGL(paged_fork_kernel<true>, dim3(1), dim3(kBook), 0, st, a);
-  else
-    hipLaunchKernelGGL(paged_fork_kernel<false>, dim3(1), dim3(kBook), 0, st, a);
-  HK_TRY(launched("paged fork launch"));
-  hipLaunchKernelGGL(paged_move_kernel, dim3(kMoveGroups), dim3(256), 0, st, moves_of(cache, a.moves, a.count, false));
-  return launched("paged fork copy launch");
+  HK_TRY(paged_launch("paged fork launch", n <= kForkLds ? paged_fork_kernel<true> : paged_fork_kernel<false>, 1, kBook, st, a));
+  return paged_launch("paged fork copy launch", paged_move_kernel, kMoveGroups, 256, st,
+                      moves_of(cache, a.moves, a.count, false));
 }
 
 int hk_paged_compact(const hk_paged_cache* cache, int32_t* table_out, int32_t* refs_out, int32_t* live_out,
@@ -764,8 +748,7 @@ int hk_paged_compact(const hk_paged_cache* cache, int32_t* table_out, int32_t* r
   a.place = w + 64;
   a.moves = reinterpret_cast<Move*>(a.place + a.pages);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(paged_compact_kernel, dim3(1), dim3(kBook), 0, st, a);
-  HK_TRY(launched("paged compact launch"));
+  HK_TRY(paged_launch("paged compact launch", paged_compact_kernel, 1, kBook, st, a));
   MoveArgs m = moves_of(cache, a.moves, a.count, true);
   m.table = cache->table;
   m.table_out = table_out;
@@ -773,8 +756,7 @@ int hk_paged_compact(const hk_paged_cache* cache, int32_t* table_out, int32_t* r
   m.place = a.place;
   m.cells = (int64_t)cache->seqs * cache->table_width;
   m.pages = a.pages;
-  hipLaunchKernelGGL(paged_move_kernel, dim3(kMoveGroups), dim3(256), 0, st, m);
-  return launched("paged move launch");
+  return paged_launch("paged move launch", paged_move_kernel, kMoveGroups, 256, st, m);
 }
 
 }  // extern "C"

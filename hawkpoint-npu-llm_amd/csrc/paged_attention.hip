@@ -1422,26 +1422,20 @@ static_assert(narrow_fits<64, false, 1>() && narrow_fits<64, true, 1>() && narro
                   narrow_fits<128, false, 2>() && narrow_fits<128, true, 2>() && wide_fits<64>() && wide_fits<128>(),
               "partial results and tickets fit the workspace");
 
-int launched() {
-  const hipError_t err = hipGetLastError();
-  return err == hipSuccess ? 0 : hip_fail(err, "paged attention launch");
-}
+constexpr char kLaunch[] = "paged attention launch";
 
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
 // most as far as the caller knows.
 template <int D, bool E4M3>
 int narrow(const PagedAttnArgs& a, int64_t rows, hipStream_t stream) {
-  if (rows <= 16)
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 1>), dim3(kCus * narrow_per_cu(D, E4M3, 1)), dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((paged_narrow_kernel<D, E4M3, 2>), dim3(kCus * narrow_per_cu(D, E4M3, 2)), dim3(kThreads), 0, stream, a);
-  return launched();
+  if (rows <= 16) return paged_launch(kLaunch, paged_narrow_kernel<D, E4M3, 1>, kCus * narrow_per_cu(D, E4M3, 1), kThreads, stream, a);
+  return paged_launch(kLaunch, paged_narrow_kernel<D, E4M3, 2>, kCus * narrow_per_cu(D, E4M3, 2), kThreads, stream, a);
 }
 
 template <int D, bool E4M3>
 int launch(PagedAttnArgs a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_new * a.group;
-  const dim3 wide_groups(kCus * wide_per_cu(D));
+  constexpr int kWideGroups = kCus * wide_per_cu(D);
   a.by_group = plan_divisor(a.group);
   a.rows_min = 1;
   a.rows_max = INT32_MAX;
@@ -1454,15 +1448,13 @@ int launch(PagedAttnArgs a, hipStream_t stream) {
     b.rows_max = few;
     a.rows_min = few + 1;
     if (few == 16) {
-      a.ticket0 = wide_groups.x;
-      a.part0 = (int)part_bytes(wide_groups.x, Narrow<D, E4M3, 1>::kPart);
-      hipLaunchKernelGGL((paged_mixed_kernel<D, E4M3>), wide_groups, dim3(kThreads), 0, stream, b, a);
-      return launched();
+      a.ticket0 = kWideGroups;
+      a.part0 = (int)part_bytes(kWideGroups, Narrow<D, E4M3, 1>::kPart);
+      return paged_launch(kLaunch, paged_mixed_kernel<D, E4M3>, kWideGroups, kThreads, stream, b, a);
     }
     if (const int rc = narrow<D, E4M3>(b, few, stream)) return rc;
   }
-  hipLaunchKernelGGL((paged_wide_kernel<D, E4M3>), wide_groups, dim3(kThreads), 0, stream, a);
-  return launched();
+  return paged_launch(kLaunch, paged_wide_kernel<D, E4M3>, kWideGroups, kThreads, stream, a);
 }
 
 }  // namespace

@@ -27,6 +27,11 @@
  * [0, table_width * page_size], a sequence outside [0, seqs) as one of length
  * 0, and `first` as values in [0, tokens].  Calls that write the same memory
  * must be ordered by the caller, as with any kernel.
+ *
+ * A call that returns HK_ERR_HIP could not make one of its launches (an error
+ * that an earlier HIP call has left is not taken for that).  After a fork, or a
+ * compaction in place, that returns it the cache is not to be used further:
+ * its tables may name pages that nobody has filled.
  */
 #ifndef HK_PAGED_H
 #define HK_PAGED_H

@@ -387,3 +387,31 @@ def test_every_block_of_every_task_has_one_workgroup(tmp_path):
                     str(tmp_path / "plan.cpp"), "-o", str(tmp_path / "plan")], check=True)
     done = subprocess.run([str(tmp_path / "plan")], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout
+
+
+# ---- errors that are not the call's own ----
+
+CHILD_STALE = CHILD[:CHILD.index("before =")] + """
+count = {"pieces": 2, "fork": 2, "compact": 2}
+p = ctypes.c_void_p()
+for name, call in calls.items():
+    # the caller's own HIP use has failed, and it has dealt with that: HIP keeps the error for the next who asks
+    fake.fake_fail_malloc_after(0)
+    assert fake.hipMalloc(ctypes.byref(p), ctypes.c_size_t(64)) != 0
+    fake.fake_fail_launch(count.get(name, 1))
+    assert call() == 0, (name, hip.last_error())
+    # all its launches were made: the next launch of all is the one to fail
+    assert calls["append"]() == hip.HK_ERR_HIP, name
+    fake.fake_fail_launch(-1)
+"""
+
+
+def test_an_earlier_hip_error_of_the_callers_stops_no_call(tmp_path):
+    """A fork that took it for its own would leave tables that name pages nobody has copied."""
+    lib = tmp_path / "libfakehip.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    str(ROOT / "tests" / "_fake_hip.cpp"), "-o", str(lib)], check=True)
+    path = os.pathsep.join([str(ROOT), str(ROOT / "hawkpoint-npu-llm_amd")])
+    done = subprocess.run([sys.executable, "-c", CHILD_STALE, str(lib)], capture_output=True, text=True, timeout=120,
+                          env={**os.environ, "PYTHONPATH": path})
+    assert done.returncode == 0, done.stdout + done.stderr
