@@ -22,6 +22,7 @@ struct AppendArgs {
   uint16_t* q_out;
   const float* cos_tab;
   const float* sin_tab;
+  const int32_t* status;  // optional: nothing is done unless its first word is HK_PAGED_DONE
   int64_t qkv_stride, q_stride;
   int q_heads;
 };
@@ -78,6 +79,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int kItems = D / 16;
   __shared__ int found;
   const int tok = blockIdx.x;
+  const int refused = a.status ? *a.status : HK_PAGED_DONE;  // (looked at below: its load is one beside those of `first`)
   if (threadIdx.x == 0) found = -1;
   __syncthreads();
   for (int e = threadIdx.x; e < a.b.n; e += 256) {
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     if (tok >= r.x && tok < r.y) found = e;
   }
   __syncthreads();
-  if (found < 0) return;
+  if (found < 0 || refused != HK_PAGED_DONE) return;
   const int2 r = entry_rows(a.b, found), s = entry_seq(a.c, a.b, found);
   const int p = s.y - r.y + tok;
   if (p < 0) return;
@@ -639,8 +641,8 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
     return HK_ERR_UNSUPPORTED;
   }
   if (n == 0 || tokens == 0) return 0;
-  AppendArgs a = {pool_of(cache, layer), {seqs, first, n, tokens}, qkv, q_out, rope_cos, rope_sin, qkv_stride,
-                  q_out_stride, q_heads};
+  AppendArgs a = {pool_of(cache, layer), {seqs, first, n, tokens}, qkv, q_out, rope_cos, rope_sin,
+                  cache->status, qkv_stride, q_out_stride, q_heads};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool e4m3 = cache->dtype == HK_PAGED_E4M3;
   const auto kernel = d == 64 ? (e4m3 ? paged_append_kernel<64, true> : paged_append_kernel<64, false>)

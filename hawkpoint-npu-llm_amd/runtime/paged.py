@@ -45,6 +45,7 @@ class PagedCache(ctypes.Structure):
         ("seqs", _i32),
         ("table_width", _i32),
         ("dtype", _i32),
+        ("status", _vp),
     ]
 
 

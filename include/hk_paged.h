@@ -18,7 +18,14 @@
  *
  * A generation step is one hk_paged_fork that makes room for the new tokens
  * (child = parent, keep = length), then per layer hk_paged_append and
- * hk_paged_attention.  The new tokens are the last ones of `length`.
+ * hk_paged_attention.  The new tokens are the last ones of `length`.  A fork
+ * that was refused leaves the lengths as they were, and an append after it
+ * would store over the last tokens of the history, in pages that other
+ * sequences may share.  So a caller who enqueues the step without a look at
+ * the fork's status words in between (or captures it) names them in
+ * cache->status: hk_paged_append then does nothing while the first of them is
+ * not HK_PAGED_DONE.  (hk_paged_attention changes no cache; after a refused
+ * fork its rows are those of the older tokens and say nothing.)
  *
  * Device contents are not seen by the host, so they are not refused but have
  * a meaning, and no memory outside the described one is touched whatever they
@@ -71,6 +78,7 @@ typedef struct hk_paged_cache {
   int32_t seqs;
   int32_t table_width;  /* pages of a sequence at most */
   int32_t dtype;        /* HK_PAGED_BF16 or HK_PAGED_E4M3 */
+  const int32_t* status; /* optional: the status words of the step's hk_paged_fork, for hk_paged_append */
 } hk_paged_cache;
 
 /* The batch of an append or an attention: entry b is sequence seqs[b] (seqs
@@ -90,7 +98,8 @@ typedef struct hk_paged_cache {
  * NULL for no rotation.  Tokens at negative positions (more rows than length)
  * are dropped, and their queries left as they were.  A sequence is listed
  * once.  Fewer than 2^24 tokens.  Pointers and strides are multiples of 16
- * bytes. */
+ * bytes.  With cache->status, neither pages nor q_out are written unless its
+ * first word is HK_PAGED_DONE. */
 int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* qkv, int64_t qkv_stride,
                     const float* rope_cos, const float* rope_sin, int32_t positions, const int32_t* seqs,
                     const int32_t* first, int32_t n, int32_t tokens, int32_t q_heads, uint16_t* q_out,

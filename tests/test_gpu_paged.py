@@ -1033,3 +1033,70 @@ def test_cache_calls_from_stream_to_stream(hk_lib):
     kv.close()
     for stream in streams:
         hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("why", ["full", "bad entry"])
+def test_a_refused_fork_stops_the_steps_appends(hk_lib, why, captured):
+    """A step enqueued in one go, and captured: after a fork that was refused the appends change neither the pages that
+    two sequences share nor the queries' memory, and once there is room the same step goes through."""
+    from runtime import hip, paged
+
+    announce(f"paged cache: a refused fork, {why}, captured {captured}")
+    rng = np.random.default_rng(81)
+    hq, hkv, dim, page = 4, 2, 64, 16
+    cache = Cache(rng, layers=2, pages=3, kv_heads=hkv, page=page, dim=dim, seqs=3, width=2, poison=False)
+    # sequence 0 and 1: one full page that they share; 2: two pages.  Two more tokens need two pages more.
+    cache.o["table"][:] = [[2, -1], [2, -1], [0, 1]]
+    cache.o["refs"][:] = (1, 1, 2)
+    cache.o["length"][:] = (16, 16, 20)
+    for layer in (0, 1):
+        cache.fill(rng, layer)
+    cache.upload()
+    x = _bits(rng.normal(size=(2, hq + 2 * hkv, dim)))
+    IN, FIRST, STATUS = _dev(x), _dev(np.array([0, 1, 2], np.int32)), _dev(np.full(2, -9, np.int32))
+    Q, GROW = _dev(np.full((2, hq, dim), 0x4242, np.uint16)), _dev(np.array([1, 1 if why == "full" else -1], np.int32))
+    SEQ = _dev(np.array([0, 1], np.int32))
+    cache.c.status = STATUS.ptr
+    handle = ctypes.c_void_p()
+    hip.check(hk_lib.hk_stream_create(ctypes.byref(handle)), "hk_stream_create")
+    stream = handle.value
+    lib, c, ws = paged.lib(), ctypes.byref(cache.c), cache.bufs["workspace"].ptr
+    _sync()
+
+    def enqueue():
+        hip.check(lib.hk_paged_fork(c, SEQ.ptr, None, None, GROW.ptr, 2, STATUS.ptr, ws, stream), "hk_paged_fork")
+        for layer in (0, 1):
+            hip.check(lib.hk_paged_append(c, layer, IN.ptr, (hq + 2 * hkv) * dim, None, None, 0, SEQ.ptr, FIRST.ptr, 2, 2, hq,
+                                          Q.ptr, hq * dim, stream), "hk_paged_append")
+
+    graph = Graph(stream) if captured else None
+    if captured:
+        with graph:
+            enqueue()
+
+    def step():
+        graph.replay() if captured else enqueue()
+        hip.check(hk_lib.hk_stream_sync(stream), "sync")
+        return tuple(STATUS.read(np.int32, 2).tolist())
+
+    for _ in range(2):
+        n = [int(v) for v in cache.o["length"][:2]]
+        grow = [1, 1 if why == "full" else -1]
+        want = oracle.fork(cache.o, [0, 1], [0, 1], n, grow)
+        assert step() == want and want[0] == (paged.FULL if why == "full" else paged.BAD_ENTRY)
+        same(cache)
+        assert np.all(Q.read(np.uint16, 2 * hq * dim) == 0x4242)
+    # room: sequence 2 is freed, and no count is below zero
+    cache.c.status = None
+    assert fork(cache, [2], [2], [0], [0]) == oracle.fork(cache.o, [2], [2], [0], [0]) == (0, 0)
+    cache.c.status = STATUS.ptr
+    GROW.write(np.array([1, 1], np.int32))
+    assert step() == oracle.fork(cache.o, [0, 1], [0, 1], [16, 16], [1, 1]) == (0, 0)
+    for layer in (0, 1):
+        want = oracle.append(cache.o, layer, _floats(x), [0, 1], [0, 1, 2], hq, None, None, lambda rows, which: rows)
+    same(cache)
+    np.testing.assert_array_equal(Q.read(np.uint16, 2 * hq * dim).reshape(2, hq, dim), _bits(want))
+    if captured:
+        graph.close()
+    hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")
