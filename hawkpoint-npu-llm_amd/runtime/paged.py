@@ -96,8 +96,8 @@ class PagedKV:
     rows of the QKV projection, ``attention`` reads them, ``compact`` moves the live pages to the front.  Activations
     are device buffers of bf16 rows; ``first`` is the list of the entries' first rows, one longer than ``seqs``.
 
-    A call waits for the one before (whatever its stream) before it hands its host arrays over: for one thread, and
-    not for capture into a graph, which is for the calls of ``lib()`` with arrays on the device.
+    A call waits for the one before (whatever its stream, which may be gone by then) before it hands its host arrays
+    over: for one thread, and not for capture into a graph, which is for the calls of ``lib()`` with arrays on the device.
     """
 
     def __init__(self, *, layers, kv_heads, head_dim, page_size, pages, seqs, table_width, dtype=BF16, k_scale=None,
@@ -126,17 +126,28 @@ class PagedKV:
                 raise ValueError(f"{name} must be [layers, kv_heads], finite and positive")
             self.bufs[name] = hip.DeviceBuffer.from_array(scale)
         hip.check(self._lib.hk_stream_sync(None), "sync")  # (the calls may go to other streams)
-        self._stream = None
+        self._start, self._done = hip.Event(), hip.Event()  # _done: the end of the call before, on its stream
+        self._start.record(None)
+        self._done.record(None)
         ptr = {name: b.ptr for name, b in self.bufs.items() if name not in ("workspace", "args")}
         self.cache = PagedCache(layer_stride=pages * page, page_stride=page, layers=layers, kv_heads=kv_heads,
                                 head_dim=head_dim, page_size=page_size, pages=pages, seqs=seqs,
                                 table_width=table_width, dtype=dtype, **ptr)
 
-    def _args(self, stream, *arrays):
-        """Device copies of a call's host arrays (None stays None), one behind the other.  The call before has read
-        its own, and is through with the workspace, when its stream is idle."""
-        hip.check(self._lib.hk_stream_sync(self._stream), "sync")
-        self._stream = stream
+    def _wait(self):
+        """For the end of the call before.  By its event: its stream is the caller's, who may have destroyed it."""
+        self._start.elapsed_ms(self._done)
+
+    def _call(self, name, *args):
+        """The last argument is the stream."""
+        rc = getattr(self._lib, name)(ctypes.byref(self.cache), *args)
+        self._done.record(args[-1])
+        hip.check(rc, name)
+
+    def _args(self, *arrays):
+        """Device copies of a call's host arrays (None stays None), one behind the other, once the call before has read
+        its own and is through with the workspace."""
+        self._wait()
         given = [a for a in arrays if a is not None]
         if sum(a.nbytes for a in given) > self.bufs["args"].nbytes:
             raise ValueError("more entries than the cache has sequences")
@@ -157,11 +168,10 @@ class PagedKV:
             return
         arrays = [_i32s(a, n, name) for a, name in ((child, "child"), (parent, "parent"), (keep, "keep"),
                                                     (grow, "grow"))]
-        args = self._args(stream, *arrays)
+        args = self._args(*arrays)
         status = self.bufs["args"].nbytes - 8
-        hip.check(self._lib.hk_paged_fork(ctypes.byref(self.cache), *args, n, self.bufs["args"].ptr + status,
-                                          self.bufs["workspace"].ptr, stream), "hk_paged_fork")
-        hip.check(self._lib.hk_stream_sync(stream), "sync")
+        self._call("hk_paged_fork", *args, n, self.bufs["args"].ptr + status, self.bufs["workspace"].ptr, stream)
+        self._wait()
         code, what = self.bufs["args"].read(np.int32, 2, status)
         if code == BAD_ENTRY:
             raise ValueError(f"fork: entry {what} is not valid")
@@ -189,35 +199,33 @@ class PagedKV:
         seqs = _i32s(seqs, n, "seqs")
         if len(np.unique(seqs)) < n:
             raise ValueError("a sequence is listed twice")
-        args = self._args(stream, seqs, first)
+        args = self._args(seqs, first)
         cos, sin, positions = rope or (None, None, 0)
         width = (q_heads + 2 * c.kv_heads) * c.head_dim
-        hip.check(self._lib.hk_paged_append(ctypes.byref(c), layer, qkv, width, cos, sin, positions, *args, n,
-                                            int(first[-1]), q_heads, q_out, q_heads * c.head_dim, stream),
-                  "hk_paged_append")
+        self._call("hk_paged_append", layer, qkv, width, cos, sin, positions, *args, n, int(first[-1]), q_heads, q_out,
+                   q_heads * c.head_dim, stream)
 
     def attention(self, layer, q, seqs, first, q_heads, out, *, scale=None, window=0, lse=None, stream=None):
         """Attention of the rows of ``q`` (device pointer), the last tokens of ``seqs``, into ``out``."""
         n, c = len(seqs), self.cache
         first = _i32s(first, n + 1, "first")
-        args = self._args(stream, _i32s(seqs, n, "seqs"), first)
+        args = self._args(_i32s(seqs, n, "seqs"), first)
         width = q_heads * c.head_dim
-        hip.check(self._lib.hk_paged_attention(ctypes.byref(c), layer, q, width, *args, n, int(first[-1]),
-                                               max(1, int(np.diff(first).max(initial=1))), q_heads,
-                                               c.head_dim ** -0.5 if scale is None else scale, window, out, width, lse,
-                                               self.bufs["workspace"].ptr, stream), "hk_paged_attention")
+        self._call("hk_paged_attention", layer, q, width, *args, n, int(first[-1]),
+                   max(1, int(np.diff(first).max(initial=1))), q_heads, c.head_dim ** -0.5 if scale is None else scale,
+                   window, out, width, lse, self.bufs["workspace"].ptr, stream)
 
     def compact(self, stream=None):
         """Moves the live pages to the front of the pool, in place; returns their number."""
-        self._args(stream)
+        self._wait()
         live = self.bufs["args"].ptr + self.bufs["args"].nbytes - 8
-        hip.check(self._lib.hk_paged_compact(ctypes.byref(self.cache), self.cache.table, self.cache.refs, live,
-                                             self.bufs["workspace"].ptr, stream), "hk_paged_compact")
-        hip.check(self._lib.hk_stream_sync(stream), "sync")
+        self._call("hk_paged_compact", self.cache.table, self.cache.refs, live, self.bufs["workspace"].ptr, stream)
+        self._wait()
         return int(self.bufs["args"].read(np.int32, 1, self.bufs["args"].nbytes - 8)[0])
 
     def _read(self, name, stream):
-        self._args(stream)
+        self._wait()
+        hip.check(self._lib.hk_stream_sync(stream), "sync")  # (the caller may have made calls of lib() there)
         return self.bufs[name].read(np.int32, self.bufs[name].nbytes // 4)
 
     def lengths(self, stream=None):

@@ -1100,3 +1100,38 @@ def test_a_refused_fork_stops_the_steps_appends(hk_lib, why, captured):
     if captured:
         graph.close()
     hip.check(hk_lib.hk_stream_destroy(stream), "hk_stream_destroy")
+
+
+def test_cache_calls_after_their_stream_is_gone(hk_lib):
+    """PagedKV's calls, each on a stream of its own that is destroyed before the next one."""
+    from runtime import hip, paged
+
+    announce("paged cache: streams that are gone")
+    rng = np.random.default_rng(91)
+    hq, hkv, dim, page = 4, 2, 64, 16
+    kv = paged.PagedKV(layers=1, kv_heads=hkv, head_dim=dim, page_size=page, pages=30, seqs=3, table_width=12)
+    x = _bits(rng.normal(size=(90, hq + 2 * hkv, dim)))
+    q = _bits(rng.normal(size=(3, hq, dim)))
+    IN, Q, OUT = _dev(x), _dev(q), _dev(np.zeros(q.shape, np.uint16))
+
+    def on_a_stream(call):
+        handle = ctypes.c_void_p()
+        hip.check(hk_lib.hk_stream_create(ctypes.byref(handle)), "hk_stream_create")
+        call(handle.value)
+        hip.check(hk_lib.hk_stream_sync(handle.value), "sync")
+        hip.check(hk_lib.hk_stream_destroy(handle.value), "hk_stream_destroy")
+
+    on_a_stream(lambda s: kv.extend([0, 1, 2], [60, 9, 21], s))
+    on_a_stream(lambda s: kv.append(0, IN.ptr, [0, 1, 2], [0, 60, 69, 90], hq, stream=s))
+    on_a_stream(lambda s: kv.attention(0, Q.ptr, [0, 1, 2], [0, 1, 2, 3], hq, OUT.ptr, stream=s))
+    on_a_stream(kv.compact)
+    assert kv.lengths().tolist() == [60, 9, 21]
+    o = {"k": np.zeros((1, 30, hkv, page, dim)), "v": np.zeros((1, 30, hkv, page, dim)),
+         "table": np.full((3, 12), -1, np.int32), "length": np.zeros(3, np.int32), "refs": np.zeros(30, np.int32)}
+    assert oracle.fork(o, range(3), range(3), [0] * 3, [60, 9, 21]) == (0, 0)
+    oracle.append(o, 0, _floats(x), range(3), [0, 60, 69, 90], hq, None, None, lambda rows, which: rows)
+    got = _floats(OUT.read(np.uint16, q.size).reshape(q.shape))
+    want, _, spread = oracle.attention(o, 0, _floats(q), range(3), range(4), dim**-0.5)
+    # (a score's float32 error is below 64 2^-24 5^2 64 / 8 < 2^-10 for these draws)
+    assert np.all(np.abs(got - want) <= 2.0**-8 * (np.abs(want) + spread) + (2.0**-9 + 2.0**-18) * spread + 1e-30)
+    kv.close()
