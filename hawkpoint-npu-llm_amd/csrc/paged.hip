@@ -1,6 +1,7 @@
 // The paged KV cache's entry points (include/hk_paged.h) and the kernels of
 // its append, fork and compaction.  The attention is in paged_attention.hip.
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "hk.h"
@@ -507,6 +508,15 @@ __global__ __launch_bounds__(kBook) void paged_compact_kernel(CompactArgs a) {
 
 // ---- checks ----
 
+// Arrays of 32-bit words.  Scalar loads leave an address's last two bits out
+// where vector loads do not, so a kernel would read two batches from one
+// misaligned array and go by both.
+int check_words(const char* who, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if ((uintptr_t)p % 4) return fail(std::string(who) + ": int32 and float32 arrays must be aligned to 4 bytes");
+  return 0;
+}
+
 int check_cache(const char* who, const hk_paged_cache* c) {
   const std::string at = std::string(who) + ": ";
   if (!c) return fail(at + "null cache");
@@ -530,11 +540,11 @@ int check_cache(const char* who, const hk_paged_cache* c) {
     return fail(at + "layer_stride below a page or not of 16 bytes");
   if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return fail(at + "pools must be aligned to 16 bytes");
   if (c->dtype == HK_PAGED_E4M3 && (!c->k_scale || !c->v_scale)) return fail(at + "e4m3 needs k_scale and v_scale");
-  return 0;
+  return check_words(who, {c->table, c->length, c->refs, c->k_scale, c->v_scale, c->status});
 }
 
-int check_batch(const char* who, const hk_paged_cache* c, int32_t layer, const int32_t* first, int32_t n,
-                int32_t tokens, int32_t q_heads) {
+int check_batch(const char* who, const hk_paged_cache* c, int32_t layer, const int32_t* seqs, const int32_t* first,
+                int32_t n, int32_t tokens, int32_t q_heads) {
   const std::string at = std::string(who) + ": ";
   if (layer < 0 || layer >= c->layers) return fail(at + "layer outside the cache");
   if (!first) return fail(at + "null pointer");
@@ -542,7 +552,7 @@ int check_batch(const char* who, const hk_paged_cache* c, int32_t layer, const i
   if (n > HK_PAGED_MAX_BATCH) return fail(at + "more than 4096 sequences in a call");
   if (q_heads <= 0 || q_heads % c->kv_heads != 0) return fail(at + "q_heads must be a positive multiple of kv_heads");
   if (q_heads > 4096) return fail(at + "more than 4096 q heads");
-  return 0;
+  return check_words(who, {seqs, first});
 }
 
 int check_rows(const char* who, const char* name, const void* p, int64_t stride, int64_t width) {
@@ -625,7 +635,7 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
                     int64_t q_out_stride, void* stream) {
   static const char who[] = "hk_paged_append";
   HK_TRY(check_cache(who, cache));
-  HK_TRY(check_batch(who, cache, layer, first, n, tokens, q_heads));
+  HK_TRY(check_batch(who, cache, layer, seqs, first, n, tokens, q_heads));
   if (!qkv) return fail("hk_paged_append: null pointer");
   const int d = cache->head_dim;
   HK_TRY(check_rows(who, "qkv", qkv, qkv_stride, (int64_t)(q_heads + 2 * cache->kv_heads) * d));
@@ -656,12 +666,13 @@ int hk_paged_attention(const hk_paged_cache* cache, int32_t layer, const uint16_
                        void* workspace, void* stream) {
   static const char who[] = "hk_paged_attention";
   HK_TRY(check_cache(who, cache));
-  HK_TRY(check_batch(who, cache, layer, first, n, tokens, q_heads));
+  HK_TRY(check_batch(who, cache, layer, seqs, first, n, tokens, q_heads));
   if (!q || !out) return fail("hk_paged_attention: null pointer");
   const int64_t width = (int64_t)q_heads * cache->head_dim;
   HK_TRY(check_rows(who, "q", q, q_stride, width));
   HK_TRY(check_rows(who, "out", out, out_stride, width));
   HK_TRY(check_workspace(who, workspace));
+  HK_TRY(check_words(who, {lse}));
   if (max_new < 1) return fail("hk_paged_attention: max_new must be positive");
   if ((int64_t)tokens * q_heads > INT32_MAX / 2) {
     set_error("hk_paged_attention: more than 2^30 rows (tokens x q_heads)");
@@ -694,6 +705,7 @@ int hk_paged_fork(const hk_paged_cache* cache, const int32_t* child, const int32
   HK_TRY(check_cache(who, cache));
   if (!status) return fail("hk_paged_fork: null status");
   HK_TRY(check_workspace(who, workspace));
+  HK_TRY(check_words(who, {child, parent, keep, grow, status}));
   if (n < 1 || n > cache->seqs) return fail("hk_paged_fork: n outside 1 .. seqs");
   ForkArgs a = {};
   a.table = cache->table;
@@ -735,6 +747,7 @@ int hk_paged_compact(const hk_paged_cache* cache, int32_t* table_out, int32_t* r
   HK_TRY(check_cache(who, cache));
   if (!table_out || !refs_out || !live_out) return fail("hk_paged_compact: null pointer");
   HK_TRY(check_workspace(who, workspace));
+  HK_TRY(check_words(who, {table_out, refs_out, live_out}));
   CompactArgs a = {};
   a.refs = cache->refs;
   a.refs_out = refs_out;

@@ -35,6 +35,8 @@
  * 0, and `first` as values in [0, tokens].  Calls that write the same memory
  * must be ordered by the caller, as with any kernel.
  *
+ * Arrays of int32 and float32 are aligned to 4 bytes, others as said below.
+ *
  * A call that returns HK_ERR_HIP could not make one of its launches (an error
  * that an earlier HIP call has left is not taken for that).  After a fork, or a
  * compaction in place, that returns it the cache is not to be used further:

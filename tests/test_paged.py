@@ -120,6 +120,21 @@ def test_refuses_bad_arguments():
             assert getattr(paged.lib(), name)(ctypes.byref(_cache()), *args.values()) == hip.HK_OK
 
 
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_refuses_misaligned_arrays(name):
+    """Vector and scalar loads would read different numbers from them."""
+    from runtime import hip, paged
+
+    for field in ("table", "length", "refs", "status"):
+        for off in (1, 2, 3):
+            _refused(name, _cache(**{field: AT + off}), hip.HK_ERR_INVALID)
+    for scales in (dict(k_scale=AT + 2, v_scale=AT), dict(k_scale=AT, v_scale=AT + 1)):
+        _refused(name, _cache(dtype=paged.E4M3, **scales), hip.HK_ERR_INVALID)
+    for arg in ("seqs", "first", "lse", "child", "parent", "keep", "grow", "status", "table_out", "refs_out", "live_out"):
+        if arg in CALLS[name]:
+            _refused(name, _cache(), hip.HK_ERR_INVALID, **{arg: AT + 2})
+
+
 CHILD = """
 import ctypes, sys
 fake = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)  # before libhk.so: its calls go here
