@@ -359,10 +359,12 @@ __device__ __forceinline__ bool next_task(const PagedAttnArgs& a, const PlanShap
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // What a product q . k is multiplied by, for powers of two.  Not zero where
-// tiny factors underflow: a hidden score is -inf times it.
+// tiny factors underflow: a hidden score is -inf times it.  Not an infinity
+// where large ones overflow: a product of 0 is a score of 0.
 template <bool E4M3>
 __device__ __forceinline__ float score_scale(const PagedAttnArgs& a, int g) {
-  return fmaxf((E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e, __builtin_bit_cast(float, 1u));
+  const float s = (E4M3 ? a.c.k_scale[g] : 1.0f) * a.scale * kLog2e;
+  return fminf(fmaxf(s, __builtin_bit_cast(float, 1u)), __FLT_MAX__);
 }
 
 // Whether one of the eight bf16 values is an infinity or NaN.

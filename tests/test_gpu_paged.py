@@ -413,6 +413,27 @@ def test_attention_with_the_smallest_scale(hk_lib, e4m3, counts):
     check_attention(*got, oracle.attention(cache.o, 0, _floats(q), [0, 1], first, 1e-45, 70), _floats(q), cache, 1e-45)
 
 
+@pytest.mark.parametrize("dim,e4m3,counts", [(64, False, (1, 2)), (128, True, (1, 1)), (64, True, (90, 40)), (128, False, (90, 1))])
+def test_attention_with_the_largest_scale(hk_lib, dim, e4m3, counts):
+    """A scale whose product with log2 e overflows: queries of zeros score 0 everywhere, so their rows are the mean of the
+    values that they see."""
+    announce(f"paged attention: largest scale, dim {dim}, e4m3 {e4m3}, rows {counts}")
+    rng = np.random.default_rng(13)
+    cache = Cache(rng, pages=20, kv_heads=1, page=16, dim=dim, seqs=2, width=10, e4m3=e4m3)
+    cache.scale = {x: np.full((1, 1), 2.0, np.float32) for x in "kv"}  # (the keys' scale adds to it)
+    if e4m3:
+        for x in "kv":
+            cache.bufs[x + "_scale"].write(cache.scale[x])
+    cache.give([150, 77], rng)
+    cache.fill(rng)
+    cache.upload()
+    first = np.cumsum([0] + list(counts))
+    q = np.zeros((first[-1], 3, dim), np.uint16)
+    got = attention(cache, 0, q, [0, 1], first, scale=3e38, window=70)
+    # (the oracle's scale does not matter to products of 0, and the tolerance's is that of the same products)
+    check_attention(*got, oracle.attention(cache.o, 0, _floats(q), [0, 1], first, 1.0, 70), _floats(q), cache, 1.0)
+
+
 @pytest.mark.parametrize("dim,e4m3,counts,lengths", [
     (64, False, (1, 1, 1), (4000, 30, 1)), (128, False, (200, 1, 60), (2000, 300, 61)), (128, True, (120,), (3500,)),
     (64, False, (40, 3, 0), (900, 2500, 5))])
