@@ -170,18 +170,14 @@ __device__ __forceinline__ PlanPlace wave_find(const PlanShape& s, const PlanEnt
 }
 
 struct Run {
-  int w;  // the run's number
-  int64_t begin, end, per;
+  PlanRun r;
   PlanPlace place;
   Entry entry;
   PlanEven even;  // splits > 0: parts of equal length instead of runs
   int task;       // of those, the workgroup's next task
 };
 
-// This workgroup's run; false: it has none.  Consecutive runs are on one XCD
-// (workgroups go round the eight), where they share K and V rows in its L2,
-// and the XCDs have equally many.
-constexpr int kXcds = 8;
+// This workgroup's run; false: it has none.
 template <bool EVEN>
 __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape& s, int least, Run& run) {
   __shared__ int64_t sums[kWaves];
@@ -189,15 +185,7 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
   __shared__ int found[5];
   const int n = a.b.n;
   run.even = {0, 0};
-  // whether unit w per lies before `total`; sets the run's number and ends
-  auto cut = [&](int64_t total) {
-    run.per = plan_per(s, total, gridDim.x, least);
-    const int runs = (int)plan_div(total + run.per - 1, run.per), share = (runs + kXcds - 1) / kXcds;
-    run.w = (int)blockIdx.x % kXcds * share + (int)blockIdx.x / kXcds;
-    run.begin = run.w * run.per;
-    run.end = min(total, run.begin + run.per);
-    return (int)blockIdx.x / kXcds < share && run.begin < run.end;
-  };
+  auto cut = [&](int64_t total) { return plan_cut(s, total, gridDim.x, least, blockIdx.x, run.r); };
   if (n == 1) {  // nothing to add up: no barrier
     run.entry = load_entry(a, 0);
     if (!takes(a, run.entry.e.count)) return false;
@@ -205,13 +193,13 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
     if constexpr (EVEN) {
       run.even = plan_even(s, run.entry.e, s.heads * head, gridDim.x);
       if (run.even.splits) {
-        run.w = (int)blockIdx.x % kXcds * ((int)gridDim.x / kXcds) + (int)blockIdx.x / kXcds;
-        run.task = run.w / run.even.splits;
+        run.r.w = plan_even_number(blockIdx.x, gridDim.x);
+        run.task = run.r.w / run.even.splits;
         return run.task < run.even.tasks;
       }
     }
     if (!cut(s.heads * head)) return false;
-    run.place = wave_find(s, run.entry.e, 0, 0, run.begin);
+    run.place = wave_find(s, run.entry.e, 0, 0, run.r.begin);
     return true;
   }
   int2 rows, seq;
@@ -236,9 +224,9 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
     const int64_t mine = units(threadIdx.x & 63), sum = wave_scan(mine);
     if (!cut(lane_of(sum, 63))) return false;
     const int64_t before = sum - mine;
-    const int l = __builtin_ctzll(__ballot(before <= run.begin && run.begin < sum));
+    const int l = __builtin_ctzll(__ballot(before <= run.r.begin && run.r.begin < sum));
     run.entry = {lane_of(seq.x, l), lane_of(rows.x, l), {lane_of(seq.y, l), lane_of(rows.y - rows.x, l)}};
-    run.place = wave_find(s, run.entry.e, l, lane_of(before, l), run.begin - lane_of(before, l));
+    run.place = wave_find(s, run.entry.e, l, lane_of(before, l), run.r.begin - lane_of(before, l));
     return true;
   }
   // (up to as many entries as threads, the units are worked out once)
@@ -263,7 +251,7 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
       mine = units(threadIdx.x);
       scan(mine, sums, chunk);
     }
-    if (before <= run.begin && run.begin < before + mine) {
+    if (before <= run.r.begin && run.r.begin < before + mine) {
       found[0] = b0 + threadIdx.x;
       found[1] = seq.x, found[2] = rows.x, found[3] = seq.y, found[4] = rows.y - rows.x;
       found_start = before;
@@ -274,23 +262,8 @@ __device__ __forceinline__ bool plan_run(const PagedAttnArgs& a, const PlanShape
   const int b = uniform(found[0]);
   const int64_t start = uniform(found_start);
   run.entry = {uniform(found[1]), uniform(found[2]), {uniform(found[3]), uniform(found[4])}};
-  run.place = wave_find(s, run.entry.e, b, start, run.begin - start);
+  run.place = wave_find(s, run.entry.e, b, start, run.r.begin - start);
   return true;
-}
-
-// On to the next task.
-__device__ __forceinline__ void plan_next(const PagedAttnArgs& a, const PlanShape& s, Run& run) {
-  PlanPlace& p = run.place;
-  p.start += plan_units(s, plan_span(s, run.entry.e, p.tile));
-  if (p.start >= run.end) return;
-  if (++p.tile < plan_tiles(s, run.entry.e)) return;
-  p.tile = 0;
-  if (++p.head < s.heads) return;
-  p.head = 0;
-  while (++p.entry < a.b.n) {
-    run.entry = load_entry(a, p.entry);
-    if (takes(a, run.entry.e.count)) return;
-  }
 }
 
 // A workgroup's part of a task: blocks [kb0, kb1) of the `rows` rows from r0 of
@@ -303,56 +276,40 @@ struct Task {
   PlanParts parts;  // of a cut task
 };
 
-// Fills in t for blocks `mine` of the task of a kv head's tile.
-__device__ __forceinline__ void set_task(const PagedAttnArgs& a, const PlanShape& s, const Entry& entry, int head, int tile,
-                                         const PlanSpan& span, const PlanBlocks& mine, Task& t) {
+// Fills in t for the workgroup's part of a task.
+__device__ __forceinline__ void set_task(const PagedAttnArgs& a, const PlanShape& s, const Entry& entry, const PlanTask& p,
+                                         Task& t) {
   t.entry = entry;
   t.table = a.c.table + (int64_t)max(entry.seq, 0) * a.c.width;
-  t.g = head;
-  t.tile = tile;
-  t.r0 = tile * s.rows;
+  t.g = p.head;
+  t.tile = p.tile;
+  t.r0 = p.tile * s.rows;
   t.rows = min(s.rows, entry.e.count * a.group - t.r0);
   t.pos0 = entry.e.length - entry.e.count;
-  t.kb0 = span.lo + mine.first;
-  t.kb1 = span.hi > span.lo ? span.lo + mine.end : t.kb0;
-  t.seen = span.seen;
+  t.kb0 = p.span.lo + p.mine.first;
+  t.kb1 = p.span.hi > p.span.lo ? p.span.lo + p.mine.end : t.kb0;
+  t.seen = p.span.seen;
+  t.cut = p.cut;
+  t.parts = p.parts;
 }
 
-// The task at the run's place, or the next one of which the run has blocks;
-// false: there is none.
+// The workgroup's next part of a task; false: there is none.
 template <bool EVEN>
 __device__ __forceinline__ bool next_task(const PagedAttnArgs& a, const PlanShape& s, Run& run, Task& t) {
   if (EVEN && run.even.splits) {
-    if (run.task >= run.even.tasks) return false;
-    const int tiles = plan_tiles(s, run.entry.e), head = uniform(run.task / tiles), tile = run.task - head * tiles;
-    const PlanSpan span = plan_span(s, run.entry.e, tile);
-    const int blocks = plan_blocks(span);
-    const PlanBlocks mine = plan_even_mine(blocks, run.even.splits, run.w - run.task * run.even.splits);
-    t.parts = {run.task * run.even.splits, plan_even_parts(blocks, run.even.splits)};
-    if (run.even.splits == 1) {
-      // (whole tasks: the workgroup's number plays no part)
-      set_task(a, s, run.entry, head, tile, span, {0, blocks}, t);
-      t.cut = false;
-    } else {
-      if (mine.first >= mine.end) return false;
-      set_task(a, s, run.entry, head, tile, span, mine, t);
-      t.cut = mine.end - mine.first < blocks;
-    }
-    run.task += run.even.splits == 1 ? (int)gridDim.x : run.even.tasks;
+    PlanTask p;
+    if (!plan_even_take(s, run.entry.e, run.even, run.r.w, gridDim.x, run.task, p)) return false;
+    set_task(a, s, run.entry, p, t);
     return true;
   }
-  for (; run.place.start < run.end; plan_next(a, s, run)) {
-    const PlanSpan span = plan_span(s, run.entry.e, run.place.tile);
-    const int blocks = plan_blocks(span);
-    const PlanBlocks mine = plan_mine(s, run.place.start, blocks, run.begin, run.end);
-    if (mine.first >= mine.end) continue;
-    set_task(a, s, run.entry, run.place.head, run.place.tile, span, mine, t);
-    t.cut = mine.end - mine.first < blocks;
-    t.parts = t.cut ? plan_parts(s, run.place.start, blocks, run.per) : PlanParts{0, 0};
-    plan_next(a, s, run);
-    return true;
-  }
-  return false;
+  return plan_take(
+      s, run.r, run.entry.e, run.place, [&](const PlanTask& p) { set_task(a, s, run.entry, p, t); },
+      [&](PlanPlace& p) {
+        while (++p.entry < a.b.n) {
+          run.entry = load_entry(a, p.entry);
+          if (takes(a, run.entry.e.count)) return;
+        }
+      });
 }
 
 // 2^(score - max): where all scores are -inf the maximum is no number to subtract.
@@ -600,7 +557,7 @@ __device__ __forceinline__ void narrow_tasks(const PagedAttnArgs& a, char* smem)
   // last.  A wave's priority falls with its progress, through the four levels
   // three times: who is behind goes first (190 chats, e4m3: 62.0 us, without 64.2;
   // 48 chats 95.4 and 96.2).
-  const int stretch = max(1, (int)min(run.per, (int64_t)INT32_MAX) / (12 * kBlockCost));
+  const int stretch = max(1, (int)min(run.r.per, (int64_t)INT32_MAX) / (12 * kBlockCost));
   int level = 3, until = stretch;
   auto step_priority = [&]() {
     if (--until > 0) return;
@@ -784,7 +741,7 @@ __device__ __forceinline__ void narrow_tasks(const PagedAttnArgs& a, char* smem)
       if (lane == 0) again[wave] = any;
     }
     const bool cut = done.cut;
-    const int slot = plan_slot(done.parts, run.w) * (N::kPart * 4);
+    const int slot = plan_slot(done.parts, run.r.w) * (N::kPart * 4);
     constexpr int kPer = D / 16;  // outputs of a thread: dimensions kPer (tid % 16) .. of row tid / 16
     const int orow = tid >> 4, od = kPer * (tid & 15);
     bool note = false;
@@ -1295,7 +1252,7 @@ __device__ __forceinline__ void wide_tasks(const PagedAttnArgs& a, char* smem) {
     const bool note = again[0] | again[1] | again[2] | again[3];
     if (cut) {
       // parts lie lane by lane: word i of thread t at 16 (i threads + t) bytes
-      const int slot = plan_slot(done.parts, run.w) * (W::kPart * 4);
+      const int slot = plan_slot(done.parts, run.r.w) * (W::kPart * 4);
       if (wave_hi >= 0) {
 #pragma unroll
         for (int i = 0; i < kQuads; ++i) {

@@ -20,6 +20,15 @@
 
 namespace hk {
 
+// A number that is the same in every lane of a wave, in a scalar register.
+HK_PLAN int plan_same(int v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_readfirstlane(v);
+#else
+  return v;
+#endif
+}
+
 // x / d for 0 <= x < 2^31 as a product: x * ceil(2^(31 + L) / d) >> (31 + L)
 // with 2^L >= d (Granlund and Montgomery, Division by invariant integers using
 // multiplication).  A division by a variable is forty instructions.
@@ -89,6 +98,24 @@ HK_PLAN int64_t plan_per(const PlanShape& s, int64_t total, int groups, int leas
   return per > most ? per : most;
 }
 
+// A workgroup's run: the units [begin, end).  Consecutive runs are on one XCD
+// (workgroups go round the eight), where they share K and V rows in its L2, and
+// the XCDs have equally many.
+constexpr int kPlanXcds = 8;
+struct PlanRun {
+  int w;  // its number
+  int64_t begin, end, per;
+};
+// The run of workgroup `block` of `groups`; false: it has none.
+HK_PLAN bool plan_cut(const PlanShape& s, int64_t total, int groups, int least, int block, PlanRun& r) {
+  r.per = plan_per(s, total, groups, least);
+  const int runs = (int)plan_div(total + r.per - 1, r.per), share = (runs + kPlanXcds - 1) / kPlanXcds;
+  r.w = block % kPlanXcds * share + block / kPlanXcds;
+  r.begin = r.w * r.per;
+  r.end = total < r.begin + r.per ? total : r.begin + r.per;
+  return block / kPlanXcds < share && r.begin < r.end;
+}
+
 // A task's place in the order: `start` units lie before it.
 struct PlanPlace {
   int entry, head, tile;
@@ -96,7 +123,8 @@ struct PlanPlace {
 };
 
 // The task that unit `rem` of entry `entry` belongs to; the entry starts at
-// unit `start`.
+// unit `start`.  (One thread's form: the kernel has the 64 lanes of a wave do
+// the same, and this is what the CPU test goes by.)
 HK_PLAN PlanPlace plan_find(const PlanShape& s, const PlanEntry& e, int entry, int64_t start, int64_t rem) {
   const int64_t per_head = plan_head_units(s, e);
   PlanPlace p = {entry, (int)plan_div(rem, per_head), 0, 0};
@@ -138,6 +166,46 @@ HK_PLAN PlanParts plan_parts(const PlanShape& s, int64_t start, int blocks, int6
 }
 HK_PLAN int plan_slot(const PlanParts& p, int w) { return 2 * w + (w == p.first ? 1 : 0); }
 
+// On to the next task of a run, if that ends later.  next(place): on to the next
+// entry that has rows, if there is one (place.entry, and e).
+template <typename Next>
+HK_PLAN void plan_next(const PlanShape& s, const PlanEntry& e, PlanPlace& p, int64_t end, Next next) {
+  p.start += plan_units(s, plan_span(s, e, p.tile));
+  if (p.start >= end) return;
+  if (++p.tile < plan_tiles(s, e)) return;
+  p.tile = 0;
+  if (++p.head < s.heads) return;
+  p.head = 0;
+  next(p);
+}
+
+// A workgroup's part of a task: the blocks `mine` of those of `span`, and the
+// parts that it is one of, if it is cut.
+struct PlanTask {
+  int head, tile;
+  PlanSpan span;
+  PlanBlocks mine;
+  PlanParts parts;
+  bool cut;
+};
+
+// The task at the place, or the next one of which the run has blocks; take(task)
+// is called before the place goes on.  False: there is none.
+template <typename Take, typename Next>
+HK_PLAN bool plan_take(const PlanShape& s, const PlanRun& r, const PlanEntry& e, PlanPlace& p, Take take, Next next) {
+  for (; p.start < r.end; plan_next(s, e, p, r.end, next)) {
+    const PlanSpan span = plan_span(s, e, p.tile);
+    const int blocks = plan_blocks(span);
+    const PlanBlocks mine = plan_mine(s, p.start, blocks, r.begin, r.end);
+    if (mine.first >= mine.end) continue;
+    const bool cut = mine.end - mine.first < blocks;
+    take(PlanTask{p.head, p.tile, span, mine, cut ? plan_parts(s, p.start, blocks, r.per) : PlanParts{0, 0}, cut});
+    plan_next(s, e, p, r.end, next);
+    return true;
+  }
+  return false;
+}
+
 // A batch of one entry over a long context may be cut another way: every task
 // into `splits` parts of as many blocks each (or, of more tasks than
 // workgroups, whole tasks dealt out one after the other), so that the
@@ -165,6 +233,27 @@ HK_PLAN PlanBlocks plan_even_mine(int blocks, int splits, int part) {
   const int parts = plan_even_parts(blocks, splits);
   if (part >= parts) return {0, 0};
   return {(int)((int64_t)blocks * part / parts), (int)((int64_t)blocks * (part + 1) / parts)};
+}
+
+// The number that workgroup `block` has in the even cut, neighbours on one XCD.
+HK_PLAN int plan_even_number(int block, int groups) { return block % kPlanXcds * (groups / kPlanXcds) + block / kPlanXcds; }
+
+// The part of task `next` that workgroup number w has, and its next task; false:
+// there is none.
+HK_PLAN bool plan_even_take(const PlanShape& s, const PlanEntry& e, const PlanEven& even, int w, int groups, int& next,
+                            PlanTask& t) {
+  if (next >= even.tasks) return false;
+  const int tiles = plan_tiles(s, e), task = next;
+  t.head = plan_same(task / tiles);
+  t.tile = task - t.head * tiles;
+  t.span = plan_span(s, e, t.tile);
+  const int blocks = plan_blocks(t.span);
+  t.parts = {task * even.splits, plan_even_parts(blocks, even.splits)};
+  // (whole tasks: the workgroup's number plays no part)
+  t.mine = even.splits == 1 ? PlanBlocks{0, blocks} : plan_even_mine(blocks, even.splits, w - task * even.splits);
+  t.cut = t.mine.end - t.mine.first < blocks;
+  next += even.splits == 1 ? groups : even.tasks;
+  return t.mine.first < t.mine.end;
 }
 
 }  // namespace hk

@@ -542,3 +542,134 @@ def test_cache_outlives_the_streams_of_its_calls(tmp_path):
     done = subprocess.run([sys.executable, "-c", CHILD_STREAMS, str(lib)], capture_output=True, text=True, timeout=120,
                           env={**os.environ, "PYTHONPATH": path})
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+# ---- the walk of the attention's workgroups ----
+
+WALK = """
+#include "paged_plan.h"
+#include <algorithm>
+#include <cstdio>
+#include <map>
+#include <random>
+#include <set>
+#include <tuple>
+#include <vector>
+using namespace hk;
+#define CHECK(x) if (!(x)) { std::printf("%s, seed %d\\n", #x, seed); return 1; }
+using Key = std::tuple<int, int, int>;  // entry, head, tile
+int main() {
+  int evens = 0, rounds = 0;
+  for (int seed = 0; seed < 1500; ++seed) {
+    std::mt19937 rng(seed);
+    auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+    const int rows[] = {16, 32, 128}, slots[] = {64, 128}, group = pick(1, 9);
+    PlanShape s{pick(1, 6), group, plan_divisor(group), pick(0, 2) ? 0 : pick(1, 300), rows[pick(0, 2)], slots[pick(0, 1)], pick(1, 3),
+                pick(0, 5)};
+    std::vector<PlanEntry> e(seed % 3 ? pick(1, 12) : 1);
+    for (auto& x : e) x = {pick(0, 3) ? pick(0, 4000) : 0, pick(0, 3) ? pick(0, 3) : pick(0, 700)};
+    if (e.size() == 1) e[0].count = pick(1, 300);
+    // the entries of one of two forms
+    const int least_rows = pick(0, 1) ? 1 : 17, most_rows = least_rows == 1 && pick(0, 1) ? 16 : INT32_MAX;
+    auto takes = [&](const PlanEntry& x) { return x.count > 0 && x.count * group >= least_rows && x.count * group <= most_rows; };
+    const int groups = 8 * pick(1, 40), n = (int)e.size(), least = pick(0, 1) ? 1 : 4;
+    int64_t total = 0;
+    std::vector<int64_t> start;
+    for (auto& x : e) start.push_back(total), total += takes(x) ? s.heads * plan_head_units(s, x) : 0;
+    std::map<Key, std::vector<std::pair<int, PlanBlocks>>> got;  // who, blocks
+    std::map<Key, int> count, ticket;
+    std::set<int> places, tickets, numbers;
+    auto arrived = [&](const Key& key, int who, const PlanTask& t, int blocks) {
+      got[key].push_back({who, t.mine});
+      if (t.mine.first >= t.mine.end || t.cut != (t.mine.end - t.mine.first < blocks)) return false;
+      if (!t.cut) return true;
+      const int place = plan_slot(t.parts, who);
+      if (place < 0 || place >= 2 * groups || !places.insert(place).second || t.parts.first < 0 || t.parts.first >= groups) return false;
+      if (!count.count(key)) {
+        count[key] = t.parts.count, ticket[key] = t.parts.first;
+        return tickets.insert(t.parts.first).second;
+      }
+      return count[key] == t.parts.count && ticket[key] == t.parts.first;
+    };
+    PlanEven even = {0, 0};
+    if (n == 1 && takes(e[0])) even = plan_even(s, e[0], total, groups);
+    for (int block = 0; block < groups; ++block) {
+      if (even.splits) {
+        const int w = plan_even_number(block, groups);
+        CHECK(w >= 0 && w < groups && numbers.insert(w).second);
+        int next = w / even.splits, parts = 0;
+        PlanTask t;
+        while (plan_even_take(s, e[0], even, w, groups, next, t)) {
+          CHECK(arrived(Key(0, t.head, t.tile), w, t, plan_blocks(t.span)));
+          CHECK(!t.cut || ++parts == 1);
+        }
+        continue;
+      }
+      PlanRun r;
+      if (!plan_cut(s, total, groups, least, block, r)) continue;
+      CHECK(numbers.insert(r.w).second && r.begin == r.w * r.per && r.end == std::min(total, r.begin + r.per));
+      int i = 0;
+      while (!(start[i] <= r.begin && takes(e[i]) && r.begin < start[i] + s.heads * plan_head_units(s, e[i]))) ++i;
+      PlanPlace p = plan_find(s, e[i], i, start[i], r.begin - start[i]);
+      PlanEntry at = e[i];
+      int parts = 0;
+      bool fine = true;
+      for (bool more = true; more;) {
+        int owner = -1;
+        more = plan_take(
+            s, r, at, p, [&](const PlanTask& t) {
+              owner = p.entry;
+              fine &= arrived(Key(owner, t.head, t.tile), r.w, t, plan_blocks(plan_span(s, e[owner], t.tile)));
+              parts += t.cut;
+            },
+            [&](PlanPlace& q) {
+              while (++q.entry < n)
+                if (takes(at = e[q.entry])) return;
+            });
+        CHECK(more == (owner >= 0));
+      }
+      CHECK(fine && parts <= 2);
+    }
+    if (!even.splits && total) {
+      // every run has a workgroup: their numbers are 0 .. with none left out
+      CHECK(!numbers.empty() && *numbers.rbegin() + 1 == (int)numbers.size());
+      const int64_t per = plan_per(s, total, groups, least);
+      CHECK((int64_t)numbers.size() == (total + per - 1) / per);
+    }
+    if (even.splits) ++evens, rounds += even.tasks > groups;
+    // every task's blocks once, its parts in the order of the workgroups, all arrived
+    size_t tasks = 0;
+    for (int i = 0; i < n; ++i) {
+      if (!takes(e[i])) continue;
+      for (int h = 0; h < s.heads; ++h)
+        for (int t = 0; t < plan_tiles(s, e[i]); ++t) {
+          const Key key(i, h, t);
+          ++tasks;
+          CHECK(got.count(key));
+          auto mine = got[key];
+          std::sort(mine.begin(), mine.end(), [](auto& a, auto& b) { return a.first < b.first; });
+          int next = 0;
+          for (size_t k = 0; k < mine.size(); ++k) {
+            CHECK(mine[k].second.first == next);
+            next = mine[k].second.end;
+            CHECK(mine.size() == 1 || mine[k].first == ticket[key] + (int)k);
+          }
+          CHECK(next == plan_blocks(plan_span(s, e[i], t)));
+          CHECK(mine.size() == 1 ? !count.count(key) : count[key] == (int)mine.size());
+        }
+    }
+    CHECK(tasks == got.size());
+  }
+  if (evens < 50 || rounds < 5) { std::printf("%d even cuts, %d of more tasks than workgroups\\n", evens, rounds); return 1; }
+}
+"""
+
+
+def test_every_workgroup_walks_its_run(tmp_path):
+    """The functions that the kernels themselves call to number the runs and go from task to task (csrc/paged_plan.h), for
+    whole launches: every task's blocks once, in parts whose places and tickets are their own and are all drawn."""
+    (tmp_path / "walk.cpp").write_text(WALK)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT / 'hawkpoint-npu-llm_amd' / 'csrc'}",
+                    str(tmp_path / "walk.cpp"), "-o", str(tmp_path / "walk")], check=True)
+    done = subprocess.run([str(tmp_path / "walk")], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout
