@@ -80,7 +80,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int kItems = D / 16;
   __shared__ int found;
   const int tok = blockIdx.x;
-  const int refused = a.status ? *a.status : HK_PAGED_DONE;  // (looked at below: its load is one beside those of `first`)
   if (threadIdx.x == 0) found = -1;
   __syncthreads();
   for (int e = threadIdx.x; e < a.b.n; e += 256) {
@@ -88,7 +87,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     if (tok >= r.x && tok < r.y) found = e;
   }
   __syncthreads();
-  if (found < 0 || refused != HK_PAGED_DONE) return;
+  if (found < 0) return;
+  if (a.status && *a.status != HK_PAGED_DONE) return;  // (in front of the search it costs calls without one 0.1 to 0.3 us)
   const int2 r = entry_rows(a.b, found), s = entry_seq(a.c, a.b, found);
   const int p = s.y - r.y + tok;
   if (p < 0) return;
