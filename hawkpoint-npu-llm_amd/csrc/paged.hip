@@ -68,13 +68,15 @@ __device__ __forceinline__ void store8(char* row, int d, const float (&x)[8], fl
 
 // One workgroup per token.  A thread takes 8 dimensions of a head's first half
 // and the 8 they turn with, 16 bytes each; the work items of a token are the q
-// heads, the k heads and the v heads times D / 16, 192 for 8 k and 32 q heads of
-// 128.  It finds the token's entry by going through all of `first`, one load a
-// thread up to 256 entries: nothing has to be planned before.  Many tokens are
-// bound by memory: pieces of 5 prompts (3205 rows, e4m3) in 14.9 us, 5.0 TB/s
-// read and written, a large copy reaches 4.7.  A decode step's 61 rows are
-// bound by the launch and four loads that wait for each other (entry, length,
-// page, row): 5.2 us a call, 3.0 of them the kernel.
+// heads, the k heads and the v heads times D / 16: 384 for 8 k and 32 q heads of
+// 128, a round and a half of the workgroup, 72 for 14 and 2 of 64.  It finds the
+// token's entry by going through all of `first`, one load a thread up to 256
+// entries: nothing has to be planned before.  Many tokens are bound by memory:
+// pieces of 5 prompts (3205 rows, e4m3) in 14.8 us, 5.0 TB/s read and written, in
+// bf16 14.2 us and 5.6 TB/s (a large copy reaches 4.7); of 14 heads on 2 of 64,
+// where a workgroup has 5 KB to move, in 5.7 us and 2.7 TB/s.  A decode step's 61
+// rows are bound by the launch and four loads that wait for each other (entry,
+// length, page, row): 4.6 to 5.5 us a call, 3.0 to 3.5 of them the kernel.
 template <int D, bool E4M3>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int kItems = D / 16;
@@ -303,7 +305,11 @@ struct ForkArgs {
 // pair the two up, and only then anything is written.  One workgroup does it
 // all, as its steps wait for each other and a barrier is cheaper than a launch
 // (4 us).  What it takes is round trips to memory, one after the other (about a
-// microsecond each, ten of them; 64 sequences, one more token each: 11 us).  So
+// microsecond each, ten of them; 64 sequences, one more token each: 11 us in a
+// pool of 2000 pages).  The pool's counts are gone through in every call, sixteen
+// waves 64 pages at a time: with 20 000 pages the step takes 13 to 16 us (the
+// copy's launch included), with 200 000 32 to 39, whether or not a page is needed.
+// So
 // the rows of all entries are gone through together, a thread per (entry,
 // column): 192 answers to 24 prompts in 17 us, where a wave per entry took 68.
 // Up to kForkLds entries are kept in LDS, more in the workspace.

@@ -5,13 +5,16 @@
 //   s_j = scale (q . k_j),  m = max s_j,  l = sum exp(s_j - m)
 //   out = sum exp(s_j - m) v_j / l,  lse = m + ln l
 // in one pass over the slots with a running maximum and sum.  The rows of all
-// query heads of a kv head are one tile's rows, so K and V are read once for
-// them.  S^T = K Q^T puts a row's scores into the lanes that hold the row's
-// column of P^T, the right operand of O^T = V^T P^T: the probabilities never
-// leave their registers.  They are rounded to bf16 there (2^-8 of each at
-// most, about what the rounding of the result costs; the three-term split of
-// the prefill kernel would triple the products), scores, maxima and sums are
-// float32.
+// query heads of a kv head are rows of the same tiles, and a tile reads K and V
+// once for all its rows (16, 32 or 128 of them).  S^T = K Q^T puts a row's
+// scores into the lanes that hold the row's column of P^T, the right operand of
+// O^T = V^T P^T: the probabilities never leave their registers.  They are
+// rounded to bf16 there, 2^-8 of each at most, about what the rounding of the
+// result costs: the results are off from float64 by 0.0017 to 0.0020 of their
+// norm, where float32 probabilities, rounded once at the end, are off by 0.0016
+// to 0.0017 (the prefill kernel's split into three bf16 terms would triple the
+// products).  Scores, maxima and sums are float32, and the sum is that of the
+// probabilities before their rounding, or lse would be off by 4e-4.
 //
 // The work of a batch is cut into equal runs of blocks (paged_plan.h), which
 // every workgroup works out by itself from the lengths on the device: a batch
@@ -380,7 +383,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_of(const PagedAttnArgs& 
 // The rows [r0, r0 + rows) of kv head g once more, a wave per row, 64 slots at a
 // time: a lane per slot for the scores, D / 64 dimensions per lane for P @ V.
 // For tasks whose tiles hold an infinity or NaN that only some of their rows
-// see: in a matrix product it would reach the others as 0 * inf.
+// see: in a matrix product it would reach the others as 0 * inf.  It is right
+// and slow: one infinity among the newest 300 values of one kv head makes a
+// piece of 701 tokens over 3003 slots take 41 ms instead of 0.07, one among the
+// newest 1000 a piece of 2039 tokens over 30011 slots 542 ms instead of 1.1, one
+// in each of 16 chats' last tokens a check of five 10 ms instead of 0.02.
 template <int D, bool E4M3>
 __device__ __forceinline__ float pool_value(const char* p, int i) {
   if constexpr (E4M3) return __builtin_amdgcn_cvt_f32_fp8(ldg(reinterpret_cast<const uint8_t*>(p) + i), 0);
@@ -435,16 +442,18 @@ __device__ __forceinline__ void rows_again(const PagedAttnArgs& a, const Entry& 
 // no barrier) with their own maxima and sums, and meet at the end of a task.
 // NQ groups of 16 rows are the MFMA's 16 columns each.
 //
-// Memory bounds it: every slot is read once, with streaming loads (7.1 TB/s in a
+// Memory bounds it: a tile reads every slot once (so entries of up to 16 NQ rows
+// read theirs once, others once per tile), with streaming loads (7.1 TB/s in a
 // plain read of 4 GiB, 6.1 without), and a tile's K and V (16 to 64 KiB per
 // workgroup) are always on the way, asked for as soon as their registers are
 // free.  48 chats of up to 9001 slots, 8 kv heads of 128, bf16 (549 MB):
 // 95.3 us, 78 at 7.1 TB/s, 6.8 TB/s inside the loop; the plan before it takes 3
 // us, the workgroups' unequal ends 5 to 10, tickets and joins 7.  190 chats in
 // e4m3 (270 MB): 62 us, 38 at that rate.  16 chats' check of five tokens (35
-// rows, 15 MB): 20 us, of these 3 to plan, 4 in the loop, 8 to join some twenty
-// parts of a task (its two tiles as one of 64 rows: 24.5 us).  One chat of 71
-// slots: 6.4 us, a launch alone 3.8.
+// rows in two tiles, 15 MB read twice): 20 us, of these 3 to plan, 4 in the loop,
+// 8 to join some twenty parts of a tile.  One tile of 64 rows instead took 24.5
+// us there, and 45.2 against 47.3 for 100 such chats of up to 9000 slots: it is
+// not kept for that twentieth.  One chat of 71 slots: 6.5 us, a launch alone 3.8.
 constexpr int kNarrowSlots = 32;
 
 template <int D, bool E4M3, int NQ>
@@ -470,7 +479,11 @@ __device__ __forceinline__ int v_key(int r) {
   return D == 128 ? 2 * (r & 7) : 2 * (((r >> 1) & 3) ^ (2 * (r & 1)));
 }
 
-// Workgroups per CU.
+// Workgroups per CU: what the registers of the loop let on it.  The e4m3 form at
+// head_dim 128 keeps seven words a lane in scratch for its third (numbers of a
+// task, read once per task; none in the loop over blocks).  With two, which
+// need no scratch, 190 chats take 58.7 us where three take 61.8, 48 chats of up
+// to 9001 slots 54.9 and 57.4.
 constexpr int narrow_per_cu(int d, bool e4m3, int nq) { return nq == 2 ? 2 : d == 64 ? 4 : e4m3 ? 3 : 2; }
 
 template <int D, bool E4M3, int NQ>
@@ -668,7 +681,9 @@ __device__ __forceinline__ void narrow_tasks(const PagedAttnArgs& a, char* smem)
       }
       if (more) load_k();
 
-      // a row sees slot s (no branches: the lanes differ)
+      // a row sees slot s.  No && and || here: the compiler made branches of
+      // them, and in a form with four groups of rows the first group's
+      // mask was wrong (the test with a window of one slot shows it).
       auto sees = [&](int n, int s) {
         return (s <= pos[n]) & (s > low[n]) & (bool)((there >> ((s >> 4) & 1)) & 1);
       };
@@ -895,8 +910,12 @@ __device__ __forceinline__ void narrow_tasks(const PagedAttnArgs& a, char* smem)
 // block.
 //
 // Products bound it, and what goes on beside them: a 2039-token piece over
-// 30011 slots, 32 q heads of 128 on 8 (0.97 TFLOP), takes 1090 to 1120 us, 870 TFLOP/s; a
-// large matrix product reaches 1160.  MFMA is busy 41% of the SIMDs' cycles, VALU
+// 30011 slots, 32 q heads of 128 on 8 (0.97 TFLOP), takes 1075 to 1145 us from
+// card to card, 850 to 900 TFLOP/s (e4m3 1052 where bf16 took 1102), and half as
+// many products at head_dim 64 take 701 (e4m3 692), 691 TFLOP/s; a large matrix
+// product reaches 1160.  At head_dim 128 the bf16 forms keep 11 to 13 words a lane
+// in scratch: numbers of a task, read once per task, none in the loop over blocks.
+// MFMA is busy 41% of the SIMDs' cycles, VALU
 // (exponentials, maxima, conversions) about as long; without the exponentials it
 // would take 5% less, without the staging of K and V 21%, without P @ V 26%: no
 // one of them is the limit.  LDS has no bank conflicts, and L2 misses are
@@ -935,6 +954,7 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// Workgroups per CU: registers at head_dim 64 let three on it.
 constexpr int wide_per_cu(int d) { return d == 64 ? 3 : 2; }
 
 template <int N>
@@ -1153,7 +1173,8 @@ __device__ __forceinline__ void wide_tasks(const PagedAttnArgs& a, char* smem) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int s = s0 + 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
-            const bool sees = (s <= pos) & (s > low) & (bool)((paged >> ((s >> 4) & 3)) & 1);  // (no branches: the lanes differ)
+            // (no && and ||, as in the narrow form: branches gave a wrong mask there)
+            const bool sees = (s <= pos) & (s > low) & (bool)((paged >> ((s >> 4) & 3)) & 1);
             sv[h][i] = sees ? sv[h][i] : -INFINITY;
           }
         };
@@ -1347,8 +1368,9 @@ __global__ __launch_bounds__(kThreads, wide_per_cu(D)) void paged_wide_kernel(Pa
 // Entries of a few rows (few) beside longer ones (many), each in its form: a
 // workgroup takes its run of the ones, then its run of the others, without
 // waiting for the workgroups that are behind.  Pieces of prompts beside chats
-// with a window: 58.6 us, in two launches 65.0; 20 sequences of up to 9000
-// slots, 7 of them with 511 new tokens, head_dim 128: 287 and 301.  (Workgroups
+// with a window took 58.6 us where two launches took 65.0 (56 to 57 now); 20
+// sequences of up to 9000 slots, 7 of them with 511 new tokens, head_dim 128: 287
+// and 301.  (Workgroups
 // that begin with the others, so that reading and products go on at the same
 // time, gain no more: 60.0 and 289.)
 constexpr int kCus = 256;
@@ -1383,6 +1405,31 @@ static_assert(narrow_fits<64, false, 1>() && narrow_fits<64, true, 1>() && narro
 
 constexpr char kLaunch[] = "paged attention launch";
 
+// Which form takes an entry goes by its rows (new tokens x heads per kv head),
+// as far as max_new says.
+//
+// Up to 64 rows in all entries: the narrow form.  Above 32 that is two tiles, and
+// it is the better one for few entries (16 chats x 35 rows, 14 heads on 2 of 64:
+// 19.6 us, wide 35.1; one of 64 rows over 30011 slots, 32 heads on 8 of 128: 62
+// and 123; four of 48 rows over 6011: 49 and 65), the worse one for many (100
+// chats of up to 9000 slots, 35 rows of 64: 65 and 59; 48 rows of 128: 434 and
+// 316; 64 rows: 448 and 318): those at head_dim 128 read more than L2 holds, and
+// each tile reads it again.  Above 64 rows wide is ahead for many as well (100
+// chats, 80 rows: 331, narrow 648; 112 rows of 64: 69 and 117).
+//
+// Long entries beside short ones: entries of up to 16 rows, a decode step's, in
+// the narrow form and all others in the wide one, one launch for both.  Entries of
+// 17 to 64 rows then get a 128-row tile; with a narrow launch of 32-row tiles of
+// their own in front, two pieces of 511 tokens beside 24 chats x 28 rows of 64
+// take 67.5 us instead of 53.5, beside 24 x 32 rows of 128 157 instead of 149,
+// beside 100 of those 270 instead of 305; one for up to 64 rows costs 16 to 28 us
+// more beside 24 chats of 35 rows.
+//
+// 17 to 32 heads per kv head: a decode step's entry has more than 16 rows, and
+// gets that launch of its own.  Two pieces of 64 tokens beside 100 chats of up to
+// 9000 slots, 24 heads per kv head of 128: 340 us, all wide 372; beside 24: 181
+// and 179; at head_dim 64 it is behind (100 chats: 121 and 104; 24: 81 and 64).
+//
 // One launch for the entries of rows_min .. rows_max rows, `rows` of them at
 // most as far as the caller knows.
 template <int D, bool E4M3>

@@ -211,7 +211,9 @@ HK_PLAN bool plan_take(const PlanShape& s, const PlanRun& r, const PlanEntry& e,
 // workgroups, whole tasks dealt out one after the other), so that the
 // workgroups of a kv head go through the same slots at the same time and find
 // them in their XCD's L2.  Equal runs start all over the context: a context that
-// L2 does not hold then comes from memory once for each tile.
+// L2 does not hold then comes from memory once for each tile.  (A 2039-token piece
+// over 30011 slots: 1113 us, in equal runs 1130 to 1230.  Two of them in a call,
+// which have equal runs: 2420 us where one has 1100; two of 1019: 1215 and 583.)
 struct PlanEven {
   int splits;  // 0: equal runs
   int tasks;

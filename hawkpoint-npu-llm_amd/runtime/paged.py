@@ -97,7 +97,8 @@ class PagedKV:
     are device buffers of bf16 rows; ``first`` is the list of the entries' first rows, one longer than ``seqs``.
 
     A call waits for the one before (whatever its stream, which may be gone by then) before it hands its host arrays
-    over: for one thread, and not for capture into a graph, which is for the calls of ``lib()`` with arrays on the device.
+    over: for one thread, and not for capture into a graph.  A program that counts microseconds keeps its arrays on the
+    device and makes the calls of ``lib()``: here each layer's append and attention waits and copies them again.
     """
 
     def __init__(self, *, layers, kv_heads, head_dim, page_size, pages, seqs, table_width, dtype=BF16, k_scale=None,
