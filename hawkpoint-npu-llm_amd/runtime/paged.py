@@ -163,7 +163,8 @@ class PagedKV:
     def fork(self, child, parent, keep, grow, stream=None):
         """Each child sequence becomes the first ``keep`` tokens of its parent with room for ``grow`` more, all at
         once; waits for the outcome.  ValueError for an entry that is not valid, RuntimeError when the pages do not
-        suffice; nothing is changed then."""
+        suffice; nothing is changed then, and the rows that were to come have no place: an append of them would store
+        over the last tokens there are."""
         n = len(child)
         if n == 0:
             return

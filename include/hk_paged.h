@@ -115,7 +115,7 @@ int hk_paged_append(const hk_paged_cache* cache, int32_t layer, const uint16_t* 
  * ln sum_j exp(scale q . k_j), by which results over parts of a context are
  * joined.  A row that sees nothing gets zeros and -inf.  Slots that a row does
  * not see have no influence on it, whatever they hold.  scale is finite and
- * positive; a score beyond float32's range is an infinity, and its row NaN.
+ * positive; a score above float32's range makes its row NaN.
  * out may be q itself, if the strides are equal.  max_new: the largest count
  * of rows of one entry, as far as the caller knows it; it chooses between
  * forms of the kernel and every value gives the same result, up to float32
